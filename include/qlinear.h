@@ -337,6 +337,87 @@ QL_API int ql_moe_combine(const float* z, const int32_t* pair_row, const float* 
                           const float* shared, long lds, const float* shared_gate, long ldg, void* out,
                           int out_dtype, long ldo, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Serving several requests from a paged key/value cache held in 4 bits. No counterpart in the
+ * reference: its cache is one request's fp32 arrays (webtorch/lm_engine.py:89-101, llm.py:1573-1616).
+ *
+ * cache: uint8 [num_pages][NKV][page / 16][ql_kv4_block_bytes(HD, group)], 16-byte aligned. A block
+ * holds 16 positions of one key/value head,
+ *   K codes [16][HD / 2] | K (s, m) [16][HD / group] | V codes [16][HD / 2] | V (s, m) [16][HD / group]
+ * two codes to a byte (LSB first), (s, m) pairs of halves. For each group of elements of a position
+ * m = half(min), s = half((max - min) / 15), n = rint((x - m) / s) in 0 .. 15, and a code stands for
+ * half(s n + m); a group with an input that is not finite (or beyond 65504) stands for nan. Slot i is
+ * position i % page of page i / page. HD is 64, 128 or 256, page a power of two from 16 to 4096, group
+ * 32, 64 or 128 and at most HD; other sizes are refused.
+ * --------------------------------------------------------------------------------------- */
+QL_API size_t ql_kv4_block_bytes(int HD, int group);   /* 0 where the sizes are not supported */
+
+/*
+ * Block tables and slot maps of one step, built on the GPU from request lengths.
+ *   prev_lens int32 [n]   tokens of each request already in the cache
+ *   new_lens  int32 [n]   tokens to append; negative: the request ends and returns its pages
+ *   table     int32 [n][table_width], row stride table_stride; row b's first ceil(prev / page) entries
+ *             are its pages. Updated in place: entries of pages that are taken.
+ *   free_pages int32 [free_capacity], n_free int32 [1]: the stack of free pages. Updated in place:
+ *             returned pages are pushed (rows in order, past free_capacity they are lost), then pages
+ *             are taken from the top; n_free_out [1] is the new height (another address than n_free).
+ * First come first served: request b is served if its pages fit the row, the sum of new_lens up to and
+ * with b is at most max_tokens, and (it needs no page, or the sum of the pages needed up to and with b
+ * is at most the height). One that is not served keeps its length and gets no tokens in this step.
+ *   seq_lens  int32 [n]   lengths after the step (0 for one that ended); another address than prev_lens
+ *   cu_new    int32 [n+1] offsets of the requests' new tokens in the step's token list
+ *   slots int64, positions int32, requests int32 [max_tokens]: of each new token; -1 past the last one
+ * The inputs are not changed otherwise, so the call gives the same outputs when it is repeated.
+ * Workspace: ql_kv_plan_workspace(n) bytes.
+ */
+QL_API size_t ql_kv_plan_workspace(int n);
+QL_API int ql_kv_plan(const int32_t* prev_lens, const int32_t* new_lens, int n, int32_t* table, long table_stride,
+               int table_width, int32_t* free_pages, int free_capacity, const int32_t* n_free, int page,
+               int max_tokens, int32_t* seq_lens, int32_t* cu_new, int64_t* slots, int32_t* positions,
+               int32_t* requests, int32_t* n_free_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * RMS norms of the query and key heads and rotate-half position embedding in one pass over QKV rows,
+ * with keys and values written to the cache in 4 bits.
+ *   qkv  [T][>= (NH + 2 NKV) HD] of dtype, row stride ld: q | k | v heads
+ *   positions int32 [T]; rope_cos, rope_sin fp32 [lmax][rot / 2]; rot a multiple of HD / 16, 0 to HD
+ *   (elements past rot are not rotated)
+ *   q_weight, k_weight  NULL (no norm) or fp32 [HD]: y = (x / sqrt(mean(x^2) + eps)) * w
+ *   q_out [T][NH][HD] of dtype
+ *   k_out [T][NKV][HD] of dtype, without a cache; or cache and slots int64 [T]: k and v are quantised
+ *   into it, and rows whose slot is outside the cache are not written.
+ * A negative position marks a padding row: zeros in q_out, nothing cached. A position of lmax or more
+ * gives nan, and nothing is cached. Every step is an IEEE fp32 operation and the mean's sum a balanced
+ * tree of neighbours, so the codes are the same wherever they are computed that way.
+ * Norm and rotation: webtorch/lm_engine.py:62-74.
+ */
+QL_API int ql_qk_norm_rope(const void* qkv, int dtype, long ld, int T, int NH, int NKV, int HD,
+                    const int32_t* positions, const float* rope_cos, const float* rope_sin, int lmax, int rot,
+                    const float* q_weight, const float* k_weight, float eps, void* q_out, void* k_out, void* cache,
+                    int num_pages, int page, int group, const int64_t* slots, void* stream);
+
+/* The values that slots [T] stand for: k_out, v_out fp16 [T][NKV][HD]; zeros for a slot outside. */
+QL_API int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, int page, int group, const int64_t* slots,
+                int T, void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention over the cache: out[t] = softmax(q[t] K^T scale) V for B requests, causal from the end of
+ * each: query i of request b is at position seq_lens[b] - q_len + i, where its queries are rows
+ * cu_q[b] .. cu_q[b + 1] - 1 of q (cu_q int32 [B + 1]), or row b when cu_q is NULL.
+ *   q [T][NH][HD] of dtype, token stride ldq (heads contiguous); out [T][NH][HD] of dtype
+ *   table int32 [B][table_width], row stride table_stride; window 0, or the number of positions that a
+ *   query sees, its own the last
+ * A row that sees no position is zero, and so are rows past cu_q[B]. A page id outside the cache or a
+ * length past the table gives nan. Scores, softmax and sums are fp32; with 16-bit inputs of more than 8
+ * rows (query tokens x NH / NKV) a request, probabilities are rounded to 11 bits, else to 22.
+ * Workspace: ql_kv4_attention_workspace(NH, NKV, HD) bytes.
+ */
+QL_API size_t ql_kv4_attention_workspace(int NH, int NKV, int HD);
+QL_API int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int NH, int NKV, int HD, const void* cache,
+                     int num_pages, int page, int group, const int32_t* table, long table_stride, int table_width,
+                     const int32_t* seq_lens, const int32_t* cu_q, int B, float scale, int window, void* out,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,6 +66,16 @@ SIGNATURES = {
     "ql_moe_act": (_c_int, [_vp, _c_long, _c_int, _vp, _c_int, _vp]),
     "ql_moe_combine": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_long, _vp, _c_long, _vp, _c_int,
                                 _c_long, _vp]),
+    "ql_kv4_block_bytes": (ctypes.c_size_t, [_c_int, _c_int]),
+    "ql_kv_plan_workspace": (ctypes.c_size_t, [_c_int]),
+    "ql_kv_plan": (_c_int, [_vp, _vp, _c_int, _vp, _c_long, _c_int, _vp, _c_int, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp,
+                            _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "ql_qk_norm_rope": (_c_int, [_vp, _c_int, _c_long, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int,
+                                 _vp, _vp, _c_float, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),
+    "ql_kv4_read": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp, _vp, _vp]),
+    "ql_kv4_attention_workspace": (ctypes.c_size_t, [_c_int, _c_int, _c_int]),
+    "ql_kv4_attention": (_c_int, [_vp, _c_int, _c_long, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _c_int, _vp,
+                                  _c_long, _c_int, _vp, _vp, _c_int, _c_float, _c_int, _vp, _vp, ctypes.c_size_t, _vp]),
 }
 
 LAUNCH_PDL = 1

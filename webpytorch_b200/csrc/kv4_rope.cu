@@ -1,0 +1,266 @@
+// Norms of queries and keys for each head, the position rotation, and the write of keys and values
+// into the paged 4-bit cache, in one pass over the QKV projection's rows.
+//
+//   r = 1 / sqrt(mean(x^2) + eps),  y = (x r) w                       (where the head has a norm)
+//   z[i] = y[i] c_i - y[i + h] s_i,  z[i + h] = y[i + h] c_i + y[i] s_i   for i < h = rot / 2
+// (rotate-half, as webtorch/lm_engine.py:66-74; elements past rot pass through). Codes of 4 bits
+// have to come out the same wherever they are made, so every step is an IEEE operation without
+// contraction and the mean's sum is a balanced tree of neighbours: x0 + x1, (x0 + x1) + (x2 + x3), ...
+// which is what lanes that hold consecutive elements and a butterfly over the lanes add up.
+#include "kv4_common.cuh"
+
+namespace ql {
+namespace {
+
+using namespace kv4;
+
+constexpr int kThreads = 128;
+
+struct RopeArgs {
+  const void* qkv;
+  long ld;
+  int T, NH, NKV;
+  const int32_t* positions;
+  const float* cos;
+  const float* sin;
+  int lmax, half;          // half = rot / 2
+  const float* qw;
+  const float* kw;
+  float eps;
+  void* q_out;
+  void* k_out;
+  uint8_t* cache;
+  long num_slots;
+  int page_shift, group;
+  const int64_t* slots;
+};
+
+template <int DT>
+__device__ __forceinline__ float ld1(const void* p, long i) {
+  return load_as_float(p, DT, i);
+}
+
+// Address of position `slot` of head g: codes of the keys (v = 0) or values (v = 1).
+__device__ __forceinline__ uint8_t* block_of(const RopeArgs& a, long slot, int g, int HD) {
+  const long page = slot >> a.page_shift;
+  const int r = (int)(slot & ((1 << a.page_shift) - 1));
+  return a.cache + ((page * a.NKV + g) << (a.page_shift - 4)) * block_bytes(HD, a.group) +
+         (long)(r >> 4) * block_bytes(HD, a.group);
+}
+
+// One warp per (token, head); lane l holds elements V l .. V l + V - 1.
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const int heads = a.NH + (a.cache || a.k_out ? (a.cache ? 2 : 1) * a.NKV : 0);
+  const long item = (long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (item >= (long)a.T * heads) return;
+  const long t = item / heads;
+  const int h = (int)(item - t * heads);
+  const bool is_q = h < a.NH, is_v = h >= a.NH + a.NKV;
+  const int pos = a.positions[t];
+  const long slot = a.cache ? a.slots[t] : -1;
+  if (!is_q && a.cache && (slot < 0 || slot >= a.num_slots || pos < 0 || pos >= a.lmax)) return;
+  float x[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = ld1<DT>(a.qkv, t * a.ld + (long)h * HD + lane * V + i);
+  if (!is_v) {
+    const float* w = is_q ? a.qw : a.kw;
+    if (w) {
+      float s[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] = __fmul_rn(x[i], x[i]);
+#pragma unroll
+      for (int n = V; n > 1; n /= 2)
+#pragma unroll
+        for (int i = 0; i < n / 2; ++i) s[i] = __fadd_rn(s[2 * i], s[2 * i + 1]);
+      float ss = s[0];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+      const float r = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[lane * V + i]);
+    }
+    const int hl = a.half / V;                       // lanes of a rotated half
+    const bool first = lane < hl, second = lane >= hl && lane < 2 * hl;
+    const int partner = first ? lane + hl : second ? lane - hl : lane;
+    const bool in = pos >= 0 && pos < a.lmax;
+    const long row = (long)(in ? pos : 0) * a.half + (second ? lane - hl : lane) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float y = __shfl_sync(0xffffffffu, x[i], partner);
+      if (first || second) {
+        const float c = a.cos[row + i], s = a.sin[row + i];
+        x[i] = first ? __fsub_rn(__fmul_rn(x[i], c), __fmul_rn(y, s)) : __fadd_rn(__fmul_rn(x[i], c), __fmul_rn(y, s));
+      }
+    }
+    // padding rows are zero; a position outside the tables gives nan
+    if (!in)
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = pos < 0 ? 0.f : __int_as_float(0x7fc00000);
+  }
+  if (is_q || !a.cache) {
+    void* out = is_q ? a.q_out : a.k_out;
+    const long at = (t * (is_q ? a.NH : a.NKV) + (is_q ? h : h - a.NH)) * HD + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) store_from_float(out, DT, at + i, x[i]);
+    return;
+  }
+  // 4 bits: minimum and range over the group's lanes
+  const int gl = a.group / V;
+  float lo = x[0], hi = x[0];
+  bool ok = true;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    ok = ok && fabsf(x[i]) <= 65504.f;               // false for nan
+  }
+  for (int o = 1; o < gl; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    ok = __shfl_xor_sync(0xffffffffu, (int)ok, o) && ok;
+  }
+  __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)), m = __float2half_rn(lo);
+  if (!ok) s = m = __ushort_as_half((unsigned short)0x7fff);
+  const float sf = __half2float(s), mf = __half2float(m);
+  uint32_t code = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float n = !ok || sf == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], mf), sf)), 0.f), 15.f);
+    code |= (uint32_t)n << (4 * i);
+  }
+  const int r = (int)(slot & 15);
+  uint8_t* blk = block_of(a, slot, is_v ? h - a.NH - a.NKV : h - a.NH, HD) +
+                 (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
+  uint8_t* cp = blk + r * (HD / 2) + lane * (V / 2);
+  if (V == 2) *cp = (uint8_t)code;
+  if (V == 4) *reinterpret_cast<uint16_t*>(cp) = (uint16_t)code;
+  if (V == 8) *reinterpret_cast<uint32_t*>(cp) = code;
+  if (lane % gl == 0)
+    reinterpret_cast<__half2*>(blk + code_bytes(HD))[r * (HD / a.group) + lane / gl] = __halves2half2(s, m);
+}
+
+// The values that slots stand for: one warp per (token, head).
+template <int HD>
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(RopeArgs a, __half* k_out, __half* v_out) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const long item = (long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (item >= (long)a.T * 2 * a.NKV) return;
+  const long t = item / (2 * a.NKV);
+  const int h = (int)(item - t * 2 * a.NKV), g = h % a.NKV;
+  const bool is_v = h >= a.NKV;
+  const long slot = a.slots[t];
+  __half* out = (is_v ? v_out : k_out) + (t * a.NKV + g) * HD + lane * V;
+  if (slot < 0 || slot >= a.num_slots) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = __ushort_as_half((unsigned short)0);
+    return;
+  }
+  const int r = (int)(slot & 15), gl = a.group / V;
+  const uint8_t* blk = block_of(a, slot, g, HD) + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
+  const uint8_t* cp = blk + r * (HD / 2) + lane * (V / 2);
+  uint32_t code = V == 2 ? *cp : V == 4 ? *reinterpret_cast<const uint16_t*>(cp) : *reinterpret_cast<const uint32_t*>(cp);
+  const __half2 sm = reinterpret_cast<const __half2*>(blk + code_bytes(HD))[r * (HD / a.group) + lane / gl];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    out[i] = __hfma(__int2half_rn((int)((code >> (4 * i)) & 15u)), __low2half(sm), __high2half(sm));
+}
+
+bool cache_args(const char* who, const void* cache, int num_pages, int NKV, int HD, int page, int group) {
+  if (!sizes_ok(NKV, HD, page, group) || num_pages <= 0 || (reinterpret_cast<uintptr_t>(cache) & 15)) {
+    set_error("%s: unsupported cache (pages=%d NKV=%d HD=%d page=%d group=%d; HD 64, 128 or 256, page a power of two "
+              "16 to 4096, group 32, 64 or 128 and at most HD, 16-byte aligned)", who, num_pages, NKV, HD, page, group);
+    return false;
+  }
+  return true;
+}
+
+template <int DT>
+cudaError_t launch_rope(const RopeArgs& a, int HD, cudaStream_t st) {
+  const long items = (long)a.T * (a.NH + (a.cache ? 2 * a.NKV : a.NKV));
+  const unsigned blocks = (unsigned)((items + kThreads / 32 - 1) / (kThreads / 32));
+  if (HD == 64) qk_norm_rope_kernel<DT, 64><<<blocks, kThreads, 0, st>>>(a);
+  else if (HD == 128) qk_norm_rope_kernel<DT, 128><<<blocks, kThreads, 0, st>>>(a);
+  else qk_norm_rope_kernel<DT, 256><<<blocks, kThreads, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace ql
+
+using namespace ql;
+
+extern "C" size_t ql_kv4_block_bytes(int HD, int group) {
+  return kv4::sizes_ok(1, HD, 16, group) ? (size_t)kv4::block_bytes(HD, group) : 0;
+}
+
+extern "C" int ql_qk_norm_rope(const void* qkv, int dtype, long ld, int T, int NH, int NKV, int HD,
+                               const int32_t* positions, const float* rope_cos, const float* rope_sin, int lmax, int rot,
+                               const float* q_weight, const float* k_weight, float eps, void* q_out, void* k_out,
+                               void* cache, int num_pages, int page, int group, const int64_t* slots, void* stream) {
+  if (T == 0) return QL_OK;
+  const int V = HD / 32;
+  if (!qkv || !positions || (rot && (!rope_cos || !rope_sin)) || !q_out || (!cache) == (!k_out) || (cache && !slots) || T < 0 ||
+      NH <= 0 || NKV <= 0 || dtype < QL_F32 || dtype > QL_BF16 || (HD != 64 && HD != 128 && HD != 256) ||
+      ld < (long)(NH + 2 * NKV) * HD || lmax <= 0 || rot < 0 || rot > HD || rot % (2 * V)) {
+    set_error("ql_qk_norm_rope: bad arguments (T=%d NH=%d NKV=%d HD=%d ld=%ld lmax=%d rot=%d dtype=%d; HD 64, 128 or "
+              "256, rot a multiple of HD / 16, either a cache with slots or k_out)", T, NH, NKV, HD, ld, lmax, rot, dtype);
+    return QL_ERR_ARG;
+  }
+  if (cache && !cache_args("ql_qk_norm_rope", cache, num_pages, NKV, HD, page, group)) return QL_ERR_ARG;
+  RopeArgs a;
+  a.qkv = qkv;
+  a.ld = ld;
+  a.T = T;
+  a.NH = NH;
+  a.NKV = NKV;
+  a.positions = positions;
+  a.cos = rope_cos;
+  a.sin = rope_sin;
+  a.lmax = lmax;
+  a.half = rot / 2;
+  a.qw = q_weight;
+  a.kw = k_weight;
+  a.eps = eps;
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.cache = reinterpret_cast<uint8_t*>(cache);
+  a.num_slots = cache ? (long)num_pages * page : 0;
+  a.page_shift = cache ? __builtin_ctz((unsigned)page) : 0;
+  a.group = group;
+  a.slots = slots;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = dtype == QL_F32 ? launch_rope<QL_F32>(a, HD, st)
+                        : dtype == QL_F16 ? launch_rope<QL_F16>(a, HD, st) : launch_rope<QL_BF16>(a, HD, st);
+  return cuda_status(e, "ql_qk_norm_rope launch");
+}
+
+extern "C" int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, int page, int group, const int64_t* slots,
+                           int T, void* k_out, void* v_out, void* stream) {
+  if (T == 0) return QL_OK;
+  if (!cache || !slots || !k_out || !v_out || T < 0) {
+    set_error("ql_kv4_read: bad arguments (T=%d)", T);
+    return QL_ERR_ARG;
+  }
+  if (!cache_args("ql_kv4_read", cache, num_pages, NKV, HD, page, group)) return QL_ERR_ARG;
+  RopeArgs a = {};
+  a.T = T;
+  a.NKV = NKV;
+  a.cache = reinterpret_cast<uint8_t*>(const_cast<void*>(cache));
+  a.num_slots = (long)num_pages * page;
+  a.page_shift = __builtin_ctz((unsigned)page);
+  a.group = group;
+  a.slots = slots;
+  const long items = (long)T * 2 * NKV;
+  const unsigned blocks = (unsigned)((items + kThreads / 32 - 1) / (kThreads / 32));
+  const cudaStream_t st = (cudaStream_t)stream;
+  __half* k = reinterpret_cast<__half*>(k_out);
+  __half* v = reinterpret_cast<__half*>(v_out);
+  if (HD == 64) kv4_read_kernel<64><<<blocks, kThreads, 0, st>>>(a, k, v);
+  else if (HD == 128) kv4_read_kernel<128><<<blocks, kThreads, 0, st>>>(a, k, v);
+  else kv4_read_kernel<256><<<blocks, kThreads, 0, st>>>(a, k, v);
+  return cuda_status(cudaGetLastError(), "ql_kv4_read launch");
+}

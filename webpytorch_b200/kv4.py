@@ -1,0 +1,196 @@
+"""Serving several requests from a paged key/value cache held in 4 bits: block tables and slot maps
+from request lengths (`plan`), the norms and rotation of queries and keys with the write into the
+cache (`qk_norm_rope`), and the attention that reads it (`attention`).
+
+The reference keeps one request's keys and values as fp32 arrays (package `webtorch`,
+lm_engine.py:89-101, llm.py:1573-1616); the norm and rotation are its `_rms`, `_rope` and `_rot`
+(lm_engine.py:62-74). The cache here is one tensor for each layer, shared by all requests in pages:
+4.5 bits a value at group 64 instead of 32. Block layout and rounding are in include/qlinear.h.
+
+A step of a batch:
+
+    p = kv4.plan(lens, new, table, free, n_free, cache.page, max_tokens)     # once a step
+    q, _ = kv4.qk_norm_rope(qkv, NH, NKV, HD, p.positions, cos, sin, cache=cache, slots=p.slots)
+    o = kv4.attention(q, cache, table, p.seq_lens, p.cu_new)                 # each layer
+
+Every call is asynchronous on the current stream (or `stream`), without a host read of any length,
+so a step can be captured in a CUDA graph.
+"""
+import math
+from collections import namedtuple
+
+import torch
+
+from . import _ffi
+from .qlinear import _device
+
+__all__ = ["KV4Cache", "Plan", "plan", "qk_norm_rope", "attention"]
+
+Plan = namedtuple("Plan", "seq_lens cu_new slots positions requests n_free")
+
+
+def _need(t, name, dtype, dim):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != dim:
+        raise TypeError("%s must be a %d-D %s tensor, got %s" % (
+            name, dim, dtype, "%s %s" % (t.dtype, tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t).__name__))
+    if not t.is_cuda:
+        raise ValueError("%s must be on the GPU" % name)
+    if dim and t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError("%s must be contiguous along its last dimension" % name)
+
+
+class KV4Cache:
+    """One layer's keys and values in 4 bits: `num_pages` pages of `page` positions for `NKV` heads of
+    `HD` elements, quantised in groups of `group` elements. `data` wraps memory that the caller owns
+    (uint8 [num_pages, NKV, page / 16, block bytes]); otherwise it is allocated, uninitialised."""
+
+    def __init__(self, num_pages, NKV, HD, page=64, group=64, device=None, data=None):
+        bb = int(_ffi.fn("ql_kv4_block_bytes")(int(HD), int(group)))
+        if not bb or page < 16 or page > 4096 or page & (page - 1) or NKV <= 0 or num_pages <= 0:
+            raise ValueError("unsupported cache: HD %s (64, 128 or 256), group %s (32, 64 or 128, at most HD), page %s "
+                             "(a power of two, 16 to 4096), %s heads, %s pages" % (HD, group, page, NKV, num_pages))
+        shape = (num_pages, NKV, page // 16, bb)
+        if data is None:
+            data = torch.empty(shape, dtype=torch.uint8, device=_device(device))
+        elif not data.is_cuda or data.dtype != torch.uint8 or tuple(data.shape) != shape or not data.is_contiguous():
+            raise ValueError("data must be a contiguous uint8 GPU tensor %s" % (shape,))
+        self.data = data
+        self.num_pages, self.NKV, self.HD, self.page, self.group = num_pages, NKV, HD, page, group
+        self.device = data.device
+        self._ws = {}
+
+    def nbytes(self):
+        return self.data.numel()
+
+    def read(self, slots, stream=None):
+        """(k, v) fp16 [T, NKV, HD]: the values that slots int64 [T] stand for; zeros for -1."""
+        _need(slots, "slots", torch.int64, 1)
+        T = slots.shape[0]
+        k = torch.empty((T, self.NKV, self.HD), dtype=torch.float16, device=self.device)
+        v = torch.empty_like(k)
+        _ffi.call("ql_kv4_read", self.data.data_ptr(), self.num_pages, self.NKV, self.HD, self.page, self.group,
+                  slots.data_ptr(), T, k.data_ptr(), v.data_ptr(), _ffi.stream_ptr(stream, self.device))
+        return k, v
+
+    def _workspace(self, NH, stream):
+        """The attention's workspace on this stream, made once: its counters are zero between calls, and
+        calls that share one may not overlap."""
+        key = (NH, _ffi.stream_ptr(stream, self.device))
+        ws = self._ws.get(key)
+        if ws is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("attention needs its workspace before a graph is captured: call it once on this "
+                                   "stream first, or pass workspace=")
+            n = int(_ffi.fn("ql_kv4_attention_workspace")(NH, self.NKV, self.HD))
+            with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(self.device)):
+                ws = self._ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        return ws
+
+
+def plan(prev_lens, new_lens, block_table, free_pages, n_free, page, max_tokens, stream=None):
+    """Block tables and slot maps of a step from request lengths, on the GPU (ql_kv_plan).
+
+    prev_lens, new_lens int32 [n]: tokens in the cache, tokens to append (negative: the request ends
+    and its pages are free again). block_table int32 [n, width] and free_pages int32 [capacity] (a
+    stack of height n_free, int32 [1]) are updated in place; lengths and the stack's height come back
+    as new tensors. Requests are served first come first served, as far as max_tokens and the free
+    pages go; one that is not keeps its length. Returns Plan(seq_lens, cu_new [n + 1], slots, positions,
+    requests [max_tokens], n_free); entries past cu_new[n] are -1."""
+    _need(prev_lens, "prev_lens", torch.int32, 1)
+    _need(new_lens, "new_lens", torch.int32, 1)
+    _need(block_table, "block_table", torch.int32, 2)
+    _need(free_pages, "free_pages", torch.int32, 1)
+    _need(n_free, "n_free", torch.int32, 1)
+    n = prev_lens.shape[0]
+    if new_lens.shape[0] != n or block_table.shape[0] != n:
+        raise ValueError("prev_lens, new_lens and block_table must have a row for each request: %d, %d, %d"
+                         % (n, new_lens.shape[0], block_table.shape[0]))
+    max_tokens = int(max_tokens)
+    dev = prev_lens.device
+    ws_bytes = int(_ffi.fn("ql_kv_plan_workspace")(n))
+    lens, cu, pos, req, left, ws = torch.empty(2 * n + 2 + 2 * max_tokens + ws_bytes // 4, dtype=torch.int32,
+                                               device=dev).split([n, n + 1, max_tokens, max_tokens, 1, ws_bytes // 4])
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    _ffi.call("ql_kv_plan", prev_lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(), block_table.stride(0),
+              block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], n_free.data_ptr(), page, max_tokens,
+              lens.data_ptr(), cu.data_ptr(), slots.data_ptr(), pos.data_ptr(), req.data_ptr(), left.data_ptr(),
+              ws.data_ptr(), ws_bytes, _ffi.stream_ptr(stream, dev))
+    return Plan(lens, cu, slots, pos, req, left)
+
+
+def qk_norm_rope(qkv, NH, NKV, HD, positions, cos, sin, *, q_weight=None, k_weight=None, eps=1e-6, cache=None,
+                 slots=None, out=None, stream=None):
+    """RMS norms of the query and key heads (where a weight fp32 [HD] is given) and rotate-half position
+    embedding over rows q | k | v of `qkv` [T, (NH + 2 NKV) HD] (ql_qk_norm_rope). cos, sin fp32
+    [lmax, rot / 2]. With a cache, keys and values are quantised into its slots int64 [T] and (q, None)
+    comes back, without one (q, k); q [T, NH, HD], k [T, NKV, HD] in qkv's dtype. A negative position is
+    padding."""
+    if qkv.dim() != 2 or qkv.shape[1] != (NH + 2 * NKV) * HD:
+        raise ValueError("qkv must be [T, %d], got %s" % ((NH + 2 * NKV) * HD, tuple(qkv.shape)))
+    _need(qkv, "qkv", qkv.dtype, 2)
+    T = qkv.shape[0]
+    _need(positions, "positions", torch.int32, 1)
+    _need(cos, "cos", torch.float32, 2)
+    _need(sin, "sin", torch.float32, 2)
+    if positions.shape[0] != T or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError("positions must be [T], cos and sin contiguous [lmax, rot / 2]")
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            _need(w, name, torch.float32, 1)
+            if w.shape[0] != HD:
+                raise ValueError("%s must be [%d]" % (name, HD))
+    q = torch.empty((T, NH, HD), dtype=qkv.dtype, device=qkv.device) if out is None else out
+    if q.dtype != qkv.dtype or tuple(q.shape) != (T, NH, HD) or not q.is_contiguous():
+        raise ValueError("out must be a contiguous %s tensor %s" % (qkv.dtype, (T, NH, HD)))
+    k = None
+    if cache is None:
+        k = torch.empty((T, NKV, HD), dtype=qkv.dtype, device=qkv.device)
+        where = (None, 0, 0, 0, None)
+    else:
+        _need(slots, "slots", torch.int64, 1)
+        if (cache.NKV, cache.HD) != (NKV, HD) or slots.shape[0] != T:
+            raise ValueError("the cache holds %d heads of %d, and slots must be [T]" % (cache.NKV, cache.HD))
+        where = (cache.data.data_ptr(), cache.num_pages, cache.page, cache.group, slots.data_ptr())
+    _ffi.call("ql_qk_norm_rope", qkv.data_ptr(), _ffi.dtype_code(qkv.dtype), max(qkv.stride(0), qkv.shape[1]), T, NH, NKV,
+              HD, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
+              _ffi.ptr(q_weight), _ffi.ptr(k_weight), float(eps), q.data_ptr(), _ffi.ptr(k), *where,
+              _ffi.stream_ptr(stream, qkv.device))
+    return q, k
+
+
+def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=0, out=None, workspace=None,
+              stream=None):
+    """softmax(q K^T scale) V over the cache for each request, causal from its end (ql_kv4_attention).
+
+    q [T, NH, HD] fp32, fp16 or bf16 (heads contiguous; tokens may be strided): rows cu_q[b] ..
+    cu_q[b + 1] - 1 are request b's last tokens (cu_q int32 [B + 1]; None: one token each). block_table
+    int32 [B, width], seq_lens int32 [B] with those tokens counted. window: positions that a query sees
+    (0: all). Rows that see nothing, and rows past cu_q[B], are zero. Returns [T, NH, HD] in q's dtype."""
+    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+        raise ValueError("q must be [T, NH, HD] with contiguous heads, got %s" % (tuple(q.shape),))
+    _need(q, "q", q.dtype, 3)
+    T, NH, HD = q.shape
+    _need(block_table, "block_table", torch.int32, 2)
+    _need(seq_lens, "seq_lens", torch.int32, 1)
+    B = seq_lens.shape[0]
+    if HD != cache.HD or NH % cache.NKV or block_table.shape[0] != B:
+        raise ValueError("q has %d heads of %d, the cache %d of %d; block_table has %d rows for %d requests"
+                         % (NH, HD, cache.NKV, cache.HD, block_table.shape[0], B))
+    if cu_q is None:
+        if T < B:
+            raise ValueError("%d queries for %d requests" % (T, B))
+    else:
+        _need(cu_q, "cu_q", torch.int32, 1)
+        if cu_q.shape[0] != B + 1:
+            raise ValueError("cu_q must be [%d]" % (B + 1))
+    if out is None:
+        out = torch.empty((T, NH, HD), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or tuple(out.shape) != (T, NH, HD) or not out.is_contiguous():
+        raise ValueError("out must be a contiguous %s tensor %s" % (q.dtype, (T, NH, HD)))
+    ws = cache._workspace(NH, stream) if workspace is None else workspace
+    _ffi.call("ql_kv4_attention", q.data_ptr(), _ffi.dtype_code(q.dtype), max(q.stride(0), NH * HD), T, NH, cache.NKV, HD,
+              cache.data.data_ptr(), cache.num_pages, cache.page, cache.group, block_table.data_ptr(),
+              max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], seq_lens.data_ptr(), _ffi.ptr(cu_q),
+              B, float(scale) if scale is not None else 1.0 / math.sqrt(HD), int(window), out.data_ptr(), ws.data_ptr(),
+              ws.numel(), _ffi.stream_ptr(stream, q.device))
+    return out
