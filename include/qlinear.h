@@ -404,13 +404,14 @@ QL_API int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, int pa
  * Attention over the cache: out[t] = softmax(q[t] K^T scale) V for B requests, causal from the end of
  * each: query i of request b is at position seq_lens[b] - q_len + i, where its queries are rows
  * cu_q[b] .. cu_q[b + 1] - 1 of q (cu_q int32 [B + 1]), or row b when cu_q is NULL.
- *   q [T][NH][HD] of dtype, token stride ldq (heads contiguous); out [T][NH][HD] of dtype
+ *   q [T][NH][HD] of dtype, token stride ldq (heads contiguous, tokens 16-byte aligned); out [T][NH][HD] of dtype
  *   table int32 [B][table_width], row stride table_stride; window 0, or the number of positions that a
  *   query sees, its own the last
  * A row that sees no position is zero, and so are rows past cu_q[B]. A page id outside the cache or a
  * length past the table gives nan. Scores, softmax and sums are fp32; with 16-bit inputs of more than 8
  * rows (query tokens x NH / NKV) a request, probabilities are rounded to 11 bits, else to 22.
- * Workspace: ql_kv4_attention_workspace(NH, NKV, HD) bytes.
+ * Workspace: ql_kv4_attention_workspace(NH, NKV, HD) bytes, 16-byte aligned, zeroed before the first call
+ * (each call leaves its counters at zero); calls that share one must not overlap. out is 8-byte aligned.
  */
 QL_API size_t ql_kv4_attention_workspace(int NH, int NKV, int HD);
 QL_API int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int NH, int NKV, int HD, const void* cache,

@@ -16,22 +16,33 @@
 // t + 4, t + 8, t + 12 of the block (the key rows are read in the order that makes it so); the words
 // of two positions are interleaved by one byte permutation per half, after which the same masks give
 // pairs of positions. Codes become the exact fp16 values they stand for: one fma each.
+// Work. A unit is one block of 16 positions of one (request, key/value head, tile); the units of all
+// requests form one line that is cut into equal pieces, one for each warp of a grid of one CTA an SM,
+// so lengths as different as they come load the GPU evenly and the host needs to know none of them.
+// A warp streams its blocks through a ring of bulk copies (one 2304-byte record a block at HD = 128, G =
+// 64), keeps the running maximum and sum of the tile, writes a tile that it holds whole, and leaves a part of
+// a tile to be joined: first with the parts of the CTA's other warps, then, for at most two tiles a
+// CTA, with those of other CTAs by whichever of them finishes last, always in the same order.
 #include "kv4_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ql {
+
+// set when a bounded wait of this file's kernel gave up (read by ql_device_status)
+__device__ int g_kv4_status = 0;
+
 namespace {
 
 using namespace kv4;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kMaxCtas = 512;   // counters in the workspace
 
 struct AttnArgs {
   const void* q;
   long ldq;
   int T, NH, NKV;
   const uint8_t* cache;
-  int num_pages, page_shift, group;
+  int num_pages, page_shift;
   const int32_t* table;
   long table_stride;
   int width;
@@ -41,86 +52,221 @@ struct AttnArgs {
   float scale;
   int window;
   void* out;
+  unsigned int* counters;   // [kMaxCtas], zero between launches
+  float* parts;             // [ctas][2 + warps] partial results
+};
+
+// Warps of a CTA by the registers that a head's state takes, and ring stages by what they leave.
+template <int HD>
+struct Shape {
+  static constexpr int kWarps = HD == 64 ? 16 : HD == 128 ? 12 : 8;
+  static constexpr int kStages = HD == 256 ? 3 : 4;
+  static constexpr int kThreads = kWarps * 32;
+};
+
+// A part of a tile: output fragments (planes summed), then m and l of 16 rows.
+template <int HD, int PL>
+struct Part {
+  static constexpr int kVec = 4 / PL;                         // floats of a lane and fragment
+  static constexpr int kStats = HD / 8 * 32 * kVec;
+  static constexpr int kFloats = kStats + 32;
+};
+template <int N>
+struct Vec;
+template <>
+struct Vec<2> { using T = float2; };
+template <>
+struct Vec<4> { using T = float4; };
+
+template <int HD, int G>
+struct Smem {
+  static constexpr int kRing = 0;
+  static constexpr int kQ = kRing + Shape<HD>::kWarps * Shape<HD>::kStages * block_bytes(HD, G);
+  static constexpr int kBar = kQ + Shape<HD>::kWarps * HD / 16 * 512;
+  static constexpr int kBytes = kBar + Shape<HD>::kWarps * Shape<HD>::kStages * 8;
 };
 
 __device__ __forceinline__ int cu(const AttnArgs& a, int b) { return a.cu_q ? min(max(a.cu_q[b], 0), a.T) : min(b, a.T); }
 
-// Splits x into fp16 high and low parts, x = hi + lo to 22 bits.
-__device__ __forceinline__ void split_h(float x, __half& hi, __half& lo) {
-  hi = __float2half_rn(x);
-  lo = __float2half_rn(x - __half2float(hi));
+struct Request {
+  int q0, ql, seq;       // first query row, queries, length
+  int tiles, blo, nblk;  // row tiles; first block that any query sees, and blocks from there
+};
+
+template <int ROWS>
+__device__ __forceinline__ Request load_request(const AttnArgs& a, int b) {
+  Request r;
+  r.q0 = cu(a, b);
+  r.ql = max(cu(a, b + 1) - r.q0, 0);
+  r.seq = max(a.seq_lens[b], 0);
+  const int end = min(r.seq, a.width << a.page_shift);
+  r.tiles = (r.ql * (a.NH / a.NKV) + ROWS - 1) / ROWS;
+  r.blo = a.window ? max(r.seq - r.ql - a.window + 1, 0) / kBlock : 0;
+  r.nblk = max((end + kBlock - 1) / kBlock - r.blo, 1);
+  return r;
+}
+
+__device__ __forceinline__ long long units_of(const Request& r, int nkv) { return (long long)r.tiles * nkv * r.nblk; }
+
+// Two floats as fp16 pairs of high and low parts, x = hi + lo to 22 bits.
+__device__ __forceinline__ void split_h2(float x, float y, __half2& hi, __half2& lo) {
+  hi = __floats2half2_rn(x, y);
+  const float2 h = __half22float2(hi);
+  lo = __floats2half2_rn(x - h.x, y - h.y);
+}
+
+// 2^x; results below 2^-126 are zero.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 template <int HD, int PL>
 struct State {
-  float o[HD / 8][4];   // C fragments of the output, tile i: element (2t, 2t + 1) * HD / 8 + i
+  float o[HD / 8][4];   // C fragments of the output, tile i: elements (2t, 2t + 1) * HD / 8 + i
   float m[3 - PL];      // running maximum of rows g (and g + 8), in units of log2
-  float l[3 - PL];      // this lane's part of the sum of exponentials
+  float l[3 - PL];      // sum of exponentials: this lane's part, the row's after reduce_rows
 };
 
-// One block of 16 positions. qf: the tile's A fragments [HD / 16][32] uint4 in shared memory.
-// coef[r] * S is the score in units of log2; lo / hi: visible positions of this lane's rows, relative
-// to the block. A masked position has p = 0, and its scales are dropped too, since memory that was
-// never written may hold codes for nan.
-template <int HD, int PL>
-__device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* blk, const uint4* qf, int group,
-                                             const float (&coef)[3 - PL], bool masked, const int (&lo)[3 - PL],
+// Queries of the tile's rows as A fragments in shared memory, and coef >= 0: coef S is the score in
+// units of log2. Rows are scaled by a power of two into fp16's range, and by the scale's sign. start()
+// runs while the loads are under way.
+template <int DT, int HD, int PL, class F>
+__device__ __forceinline__ void load_queries(const AttnArgs& a, const Request& r, int kvh, int r0, int nrows, int grp,
+                                             uint4* qf, float (&coef)[3 - PL], const F& start) {
+  constexpr int WV = DT == QL_F32 ? 8 : 4;       // words of 8 elements
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint32_t raw[3 - PL][HD / 32 * WV];
+#pragma unroll
+  for (int k = 0; k < 3 - PL; ++k) {
+    const int i = r0 + min(g + 8 * k, nrows - 1);   // rows past the tile repeat its last one
+    const long at = (long)(r.q0 + i / grp) * a.ldq + (long)(kvh * grp + i % grp) * HD + t * (HD / 4);
+    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.q) + at * (DT == QL_F32 ? 4 : 2));
+#pragma unroll
+    for (int j = 0; j < HD / 32 * WV / 4; ++j) {
+      const uint4 u = p[j];
+      raw[k][4 * j] = u.x; raw[k][4 * j + 1] = u.y; raw[k][4 * j + 2] = u.z; raw[k][4 * j + 3] = u.w;
+    }
+  }
+  start();
+  const auto element = [&](int k, int i) -> float {
+    if (DT == QL_F32) return __int_as_float(raw[k][i]);
+    const uint32_t u = raw[k][i / 2];
+    if (DT == QL_F16) return i & 1 ? __high2float(u32_as_h2(u)) : __low2float(u32_as_h2(u));
+    return __int_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+  };
+  float inv[3 - PL];
+#pragma unroll
+  for (int k = 0; k < 3 - PL; ++k) {
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) mx = fmaxf(mx, fabsf(element(k, i)));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const int e = stage_exponent(mx);
+    inv[k] = copysignf(exp2i(-e), a.scale);
+    coef[k] = exp2i(e) * (fabsf(a.scale) * 1.4426950408889634f);
+  }
+#pragma unroll
+  for (int w = 0; w < HD / 32; ++w)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // the pairs that the nibble masks of a key word give: (0, 4), (1, 5) | (2, 6), (3, 7); row g (its
+      // high part) and row g + 8 (row g's low part)
+      __half2 f[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = 8 * w + 2 * h + j;
+        if (PL == 2) {
+          split_h2(element(0, i) * inv[0], element(0, i + 4) * inv[0], f[0][j], f[1][j]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 3 - PL; ++k)
+            f[k][j] = __floats2half2_rn(element(k, i) * inv[k], element(k, i + 4) * inv[k]);
+        }
+      }
+      qf[(2 * w + h) * 32 + lane] = make_uint4(h2_as_u32(f[0][0]), h2_as_u32(f[1][0]), h2_as_u32(f[0][1]), h2_as_u32(f[1][1]));
+    }
+}
+
+// The running maximum is moved (and the sums with it) when it grows by more than 2^kLazy, not each
+// time: p' stays within fp16 and the ratio o / l does not depend on it. At 80 blocks a warp a row's
+// maximum grows in about a third of them.
+constexpr float kLazy = 6.f;
+constexpr float kPShift = 9.f;   // p' = 2^9 p, up to 2^15: 11 bits of probabilities down to 2^-23
+
+// One block of 16 positions in shared memory. MASKED: some of its positions are not seen by some row.
+// lo / hi: visible positions of this lane's rows, relative to the block; any_lo / any_hi: of any row.
+// A masked position has p = 0, and where no row sees it its scales are dropped too, since memory that
+// was never written may hold codes for nan.
+template <int HD, int G, int PL, bool MASKED>
+__device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* blk, const uint4* qf,
+                                             const float (&coef)[3 - PL], const int (&lo)[3 - PL],
                                              const int (&hi)[3 - PL], int any_lo, int any_hi) {
   constexpr int R = 3 - PL;                 // rows of a lane
   constexpr int KW = HD / 32, VW = HD / 64; // words of a lane: keys of one position, values of one
+  constexpr int NG = HD / G;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int ng = HD / group;
   const uint8_t* ks = blk + code_bytes(HD);
-  const uint8_t* vc = ks + scale_bytes(HD, group);
+  const uint8_t* vc = ks + scale_bytes(HD, G);
   const uint8_t* vs = vc + code_bytes(HD);
-  float z[R][4];                            // positions t, t + 4, t + 8, t + 12
+  float c[2][4] = {};                       // S of positions t, t + 4 | t + 8, t + 12
+  {
+    uint32_t w[2][KW];
+    __half2 sm[2][HD == 256 && G == 32 ? 2 : 1];   // a lane's elements are in one group, or two
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int row = 8 * j + (g >> 1) + 4 * (g & 1);
-    uint32_t w[KW];
-#pragma unroll
-    for (int i = 0; i < KW; i += (KW >= 4 ? 4 : 2)) {
+    for (int j = 0; j < 2; ++j) {
+      const int row = 8 * j + (g >> 1) + 4 * (g & 1);
+      const uint8_t* kp = blk + row * (HD / 2) + t * (HD / 8);
       if constexpr (KW >= 4) {
-        const uint4 u = *reinterpret_cast<const uint4*>(blk + row * (HD / 2) + t * (HD / 8) + i * 4);
-        w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
+#pragma unroll
+        for (int i = 0; i < KW; i += 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(kp + 4 * i);
+          w[j][i] = u.x; w[j][i + 1] = u.y; w[j][i + 2] = u.z; w[j][i + 3] = u.w;
+        }
       } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(blk + row * (HD / 2) + t * (HD / 8) + i * 4);
-        w[i] = u.x; w[i + 1] = u.y;
+        const uint2 u = *reinterpret_cast<const uint2*>(kp);
+        w[j][0] = u.x; w[j][1] = u.y;
       }
+#pragma unroll
+      for (int i = 0; i < (HD == 256 && G == 32 ? 2 : 1); ++i)
+        sm[j][i] = reinterpret_cast<const __half2*>(ks)[row * NG + (t * (HD / 4) + 32 * i) / G];
     }
-    float c[4] = {0.f, 0.f, 0.f, 0.f};
-    __half2 s2, m2;
 #pragma unroll
     for (int i = 0; i < KW; ++i) {
-      if (i == 0 || HD == 256) {            // at HD = 256 a lane's 64 elements may span two groups
-        const __half2 sm = reinterpret_cast<const __half2*>(ks)[row * ng + (t * (HD / 4) + 8 * i) / group];
-        s2 = __low2half2(sm);
-        m2 = __high2half2(sm);
-      }
-      __half2 n[4];
-      codes_h2(w[i], n);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) n[k] = __hfma2(n[k], s2, m2);
       const uint4 a0 = qf[(2 * i) * 32 + lane], a1 = qf[(2 * i + 1) * 32 + lane];
-      mma_16816_f16(c, a0.x, a0.y, a0.z, a0.w, h2_as_u32(n[0]), h2_as_u32(n[1]));
-      mma_16816_f16(c, a1.x, a1.y, a1.z, a1.w, h2_as_u32(n[2]), h2_as_u32(n[3]));
-    }
-    if (PL == 2) {
-      z[0][2 * j] = (c[0] + c[2]) * coef[0];
-      z[0][2 * j + 1] = (c[1] + c[3]) * coef[0];
-    } else {
-      z[0][2 * j] = c[0] * coef[0];
-      z[0][2 * j + 1] = c[1] * coef[0];
-      z[R - 1][2 * j] = c[2] * coef[R - 1];
-      z[R - 1][2 * j + 1] = c[3] * coef[R - 1];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const __half2 u = sm[j][HD == 256 && G == 32 ? i / 4 : 0], s2 = __low2half2(u), m2 = __high2half2(u);
+        __half2 n[4];
+        codes_h2(w[j][i], n);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) n[k] = __hfma2(n[k], s2, m2);
+        mma_16816_f16(c[j], a0.x, a0.y, a0.z, a0.w, h2_as_u32(n[0]), h2_as_u32(n[1]));
+        mma_16816_f16(c[j], a1.x, a1.y, a1.z, a1.w, h2_as_u32(n[2]), h2_as_u32(n[3]));
+      }
     }
   }
-  if (masked)
+  float z[R][4];                            // of positions t + 4 k
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (PL == 2) {
+        z[0][2 * j + k] = c[j][k] + c[j][k + 2];
+      } else {
+        z[0][2 * j + k] = c[j][k];
+        z[R - 1][2 * j + k] = c[j][k + 2];
+      }
+    }
+  if (MASKED) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (t + 4 * k < lo[r] || t + 4 * k >= hi[r]) z[r][k] = -INFINITY;
+  }
   float mn[R];
   bool grows = false;
 #pragma unroll
@@ -128,15 +274,16 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
     float x = fmaxf(fmaxf(z[r][0], z[r][1]), fmaxf(z[r][2], z[r][3]));
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-    mn[r] = fmaxf(st.m[r], x);
-    grows = grows || mn[r] > st.m[r];
+    mn[r] = MASKED && x == -INFINITY ? -INFINITY : x * coef[r];   // coef may be 0
+    grows = grows || mn[r] > st.m[r] + kLazy;                     // st.m = -inf: the first one
   }
   if (__any_sync(0xffffffffu, grows)) {
     float f[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      f[r] = mn[r] > st.m[r] ? exp2f(st.m[r] - mn[r]) : 1.f;
-      st.m[r] = mn[r];
+      const float top = fmaxf(st.m[r], mn[r]);
+      f[r] = top > st.m[r] ? ex2(st.m[r] - top) : 1.f;
+      st.m[r] = top;
       st.l[r] *= f[r];
     }
 #pragma unroll
@@ -147,52 +294,56 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
       st.o[i][3] *= f[R - 1];
     }
   }
-  // p' = 2^11 p: fp16 keeps 11 bits of probabilities down to 2^-25
   uint32_t a[4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    float p[R][2];
+  for (int r = 0; r < R; ++r) {
+    const float base = kPShift - (MASKED && st.m[r] == -INFINITY ? 0.f : st.m[r]);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float base = (st.m[r] == -INFINITY ? 0.f : st.m[r]) - 11.f;
+    for (int j = 0; j < 2; ++j) {
+      float p[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        p[r][k] = exp2f(z[r][2 * j + k] - base);
-        st.l[r] += p[r][k];
+        p[k] = ex2(fmaf(z[r][2 * j + k], coef[r], base));
+        // a masked position, where coef is 0
+        if (MASKED && z[r][2 * j + k] == -INFINITY) p[k] = 0.f;
+        st.l[r] += p[k];
       }
-    }
-    if (PL == 2) {
-      __half h0, l0, h1, l1;
-      split_h(p[0][0], h0, l0);
-      split_h(p[0][1], h1, l1);
-      a[2 * j] = h2_as_u32(__halves2half2(h0, h1));
-      a[2 * j + 1] = h2_as_u32(__halves2half2(l0, l1));
-    } else {
-      a[2 * j] = h2_as_u32(__floats2half2_rn(p[0][0], p[0][1]));
-      a[2 * j + 1] = h2_as_u32(__floats2half2_rn(p[R - 1][0], p[R - 1][1]));
+      if (PL == 2) {
+        __half2 h, l;
+        split_h2(p[0], p[1], h, l);
+        a[2 * j] = h2_as_u32(h);
+        a[2 * j + 1] = h2_as_u32(l);
+      } else {
+        a[2 * j + r] = h2_as_u32(__floats2half2_rn(p[0], p[1]));
+      }
     }
   }
   // values: words of positions t, t + 4 | t + 8, t + 12, elements g HD / 8 ...
   uint32_t w[4][VW];
-  __half2 s2[2], m2[2];
+  __half2 s2[2], m2[2], sm[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const uint8_t* p = vc + (t + 4 * k) * (HD / 2) + g * (HD / 16);
-#pragma unroll
-    for (int i = 0; i < VW; ++i) w[k][i] = reinterpret_cast<const uint32_t*>(p)[i];
+    if constexpr (VW == 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
+    } else if constexpr (VW == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[k][0] = u.x; w[k][1] = u.y;
+    } else {
+      w[k][0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+    sm[k] = reinterpret_cast<const __half2*>(vs)[(t + 4 * k) * NG + g * (HD / 8) / G];
   }
-  {
-    __half2 sm[4];
+  if (MASKED) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      sm[k] = reinterpret_cast<const __half2*>(vs)[(t + 4 * k) * ng + g * (HD / 8) / group];
-      if (masked && (t + 4 * k < any_lo || t + 4 * k >= any_hi)) sm[k] = h2_const(0u);
-    }
+    for (int k = 0; k < 4; ++k)
+      if (t + 4 * k < any_lo || t + 4 * k >= any_hi) sm[k] = h2_const(0u);
+  }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      s2[k] = __lows2half2(sm[2 * k], sm[2 * k + 1]);
-      m2[k] = __highs2half2(sm[2 * k], sm[2 * k + 1]);
-    }
+  for (int k = 0; k < 2; ++k) {
+    s2[k] = __lows2half2(sm[2 * k], sm[2 * k + 1]);
+    m2[k] = __highs2half2(sm[2 * k], sm[2 * k + 1]);
   }
 #pragma unroll
   for (int i = 0; i < VW; ++i)
@@ -200,8 +351,8 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
     for (int h = 0; h < 2; ++h) {
       const uint32_t sel = h ? 0x7632u : 0x5410u;
       __half2 b0[4], b1[4];
-      // nibbles 0..3 of the half word: codes_h2 reads them as (nibble j, nibble j + 4) of the
-      // interleaved word, which are the two positions
+      // nibbles 0..3 of the half words of two positions: codes_h2 reads the interleaved word as
+      // (nibble j of one, nibble j of the other)
       codes_h2(__byte_perm(w[0][i], w[1][i], sel), b0);
       codes_h2(__byte_perm(w[2][i], w[3][i], sel), b1);
 #pragma unroll
@@ -213,182 +364,577 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
     }
 }
 
-// The request and the first row of tile x. Tiles of request b start at cu[b] grp / rows + b, which
-// leaves room for ceil(rows of b / rows) of them wherever the division falls.
-__device__ __forceinline__ int tile_start(const AttnArgs& a, int b, int grp, int rows) {
-  return (int)((long)cu(a, b) * grp / rows) + b;
+template <int HD, int PL>
+__device__ __forceinline__ void store_part(const State<HD, PL>& st, float* part) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) {
+    if (PL == 2)
+      reinterpret_cast<float2*>(part)[i * 32 + lane] = make_float2(st.o[i][0] + st.o[i][2], st.o[i][1] + st.o[i][3]);
+    else
+      reinterpret_cast<float4*>(part)[i * 32 + lane] = make_float4(st.o[i][0], st.o[i][1], st.o[i][2], st.o[i][3]);
+  }
+  float* ml = part + Part<HD, PL>::kStats;
+  if ((lane & 3) == 0)
+#pragma unroll
+    for (int r = 0; r < 3 - PL; ++r) {
+      ml[(lane >> 2) + 8 * r] = st.m[r];
+      ml[16 + (lane >> 2) + 8 * r] = st.l[r];
+    }
+}
+
+template <int HD, int PL>
+__device__ __forceinline__ void copy_part(float* to, const float* from) {
+  for (int i = threadIdx.x & 31; i < Part<HD, PL>::kFloats / 4; i += 32)
+    reinterpret_cast<float4*>(to)[i] = reinterpret_cast<const float4*>(from)[i];
+}
+
+// st joined with n parts in shared memory, in their order.
+template <int HD, int PL>
+__device__ __forceinline__ void join_parts(State<HD, PL>& st, const float* part, int n) {
+  constexpr int SIZE = Part<HD, PL>::kFloats;
+  const int lane = threadIdx.x & 31;
+  float top[3 - PL], f[3 - PL];
+#pragma unroll
+  for (int r = 0; r < 3 - PL; ++r) {
+    const float* ml = part + Part<HD, PL>::kStats + (lane >> 2) + 8 * r;
+    top[r] = st.m[r];
+    for (int p = 0; p < n; ++p) top[r] = fmaxf(top[r], ml[p * SIZE]);
+    const float base = top[r] == -INFINITY ? 0.f : top[r];
+    f[r] = ex2(st.m[r] - base);
+    st.m[r] = top[r];
+    st.l[r] *= f[r];
+    top[r] = base;
+  }
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) {
+    st.o[i][0] *= f[0];
+    st.o[i][1] *= f[0];
+    st.o[i][2] *= f[2 - PL];
+    st.o[i][3] *= f[2 - PL];
+  }
+  for (int p = 0; p < n; ++p, part += SIZE) {
+#pragma unroll
+    for (int r = 0; r < 3 - PL; ++r) {
+      const float* ml = part + Part<HD, PL>::kStats + (lane >> 2) + 8 * r;
+      f[r] = ex2(ml[0] - top[r]);
+      st.l[r] = fmaf(f[r], ml[16], st.l[r]);
+    }
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) {
+      const auto v = reinterpret_cast<const typename Vec<4 / PL>::T*>(part)[i * 32 + lane];
+      st.o[i][0] = fmaf(f[0], v.x, st.o[i][0]);
+      st.o[i][1] = fmaf(f[0], v.y, st.o[i][1]);
+      if constexpr (PL == 1) {
+        st.o[i][2] = fmaf(f[1], v.z, st.o[i][2]);
+        st.o[i][3] = fmaf(f[1], v.w, st.o[i][3]);
+      }
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store2(void* out, long i, float x, float y) {
+  if (DT == QL_F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(out) + i) = make_float2(x, y);
+  else if (DT == QL_F16) *reinterpret_cast<__half2*>(reinterpret_cast<__half*>(out) + i) = __floats2half2_rn(x, y);
+  else *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(out) + i) = __floats2bfloat162_rn(x, y);
+}
+
+// Output rows of a tile: row i is token q0 + i / grp, head kvh grp + i % grp.
+__device__ __forceinline__ long out_row(const AttnArgs& a, int q0, int kvh, int row, int grp) {
+  return (long)(q0 + row / grp) * a.NH + kvh * grp + row % grp;
 }
 
 template <int DT, int HD, int PL>
-__global__ void __launch_bounds__(kThreads) kv4_attention_kernel(AttnArgs a) {
-  constexpr int R = 3 - PL, ROWS = 16 / PL;
-  __shared__ uint4 qf[HD / 16][32];
-  __shared__ float qexp[ROWS];
-  __shared__ float red_m[kWarps][ROWS], red_l[kWarps][ROWS];
-  __shared__ float red_o[kWarps][ROWS][HD];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int grp = a.NH / a.NKV, kvh = blockIdx.y, x = blockIdx.x;
-  int b = 0;
-  for (int hi = a.B - 1; b < hi;) {   // the last b whose first tile is at or before x
-    const int mid = (b + hi + 1) >> 1;
-    if (tile_start(a, mid, grp, ROWS) <= x) b = mid;
-    else hi = mid - 1;
-  }
-  const int q0 = cu(a, b), ql = max(cu(a, b + 1) - q0, 0);
-  const int r0 = (x - tile_start(a, b, grp, ROWS)) * ROWS;
-  const int nrows = min(ROWS, ql * grp - r0);
-  if (nrows <= 0) return;
-  // queries: row r of the tile is token q0 + (r0 + r) / grp, head kvh grp + (r0 + r) % grp
-  for (int r = warp; r < ROWS; r += kWarps) {
-    float mx = 0.f;
-    const int i = r0 + r;
-    const long at = (long)(q0 + i / grp) * a.ldq + (long)(kvh * grp + i % grp) * HD;
-    if (r < nrows)
-      for (int d = lane; d < HD; d += 32) mx = fmaxf(mx, fabsf(load_as_float(a.q, DT, at + d)));
+__device__ __forceinline__ void write_tile(const AttnArgs& a, const State<HD, PL>& st, int q0, int kvh, int r0,
+                                           int nrows, int grp) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const int e = stage_exponent(mx);
-    if (lane == 0) qexp[r] = exp2i(e);
-    const float inv = exp2i(-e);
-    for (int d = lane; d < HD; d += 32) {
-      const float v = r < nrows ? load_as_float(a.q, DT, at + d) * inv : 0.f;
-      __half hi, lo;
-      split_h(v, hi, lo);
-      // element d: lane t = d / (HD / 4), word w, nibble j; fragment 2 w + (j & 2) / 2, registers
-      // 0 / 1 (k pair 0) or 2 / 3 (k pair 1) by j & 1, half by j >> 2
-      const int tt = d / (HD / 4), w = (d % (HD / 4)) / 8, j = d & 7;
-      __half* f = reinterpret_cast<__half*>(&qf[2 * w + ((j >> 1) & 1)][(r & 7) * 4 + tt]);
-      const int reg = 2 * (j & 1), half = j >> 2;
-      if (PL == 2) {
-        f[reg * 2 + half] = hi;
-        f[(reg + 1) * 2 + half] = lo;
-      } else {
-        f[(reg + (r >> 3)) * 2 + half] = hi;
+  for (int r = 0; r < 3 - PL; ++r) {
+    if (g + 8 * r >= nrows) continue;
+    const float inv = st.l[r] == 0.f ? 0.f : 1.f / st.l[r];   // a row that sees nothing is zero
+    const long at = out_row(a, q0, kvh, r0 + g + 8 * r, grp) * HD + t * (HD / 4);
+    // the lane's HD / 4 elements are consecutive: tile i holds elements i and HD / 8 + i of them
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < HD / 8; i += 2) {
+        const float x = (PL == 2 ? st.o[i][k] + st.o[i][k + 2] : st.o[i][2 * r + k]) * inv;
+        const float y = (PL == 2 ? st.o[i + 1][k] + st.o[i + 1][k + 2] : st.o[i + 1][2 * r + k]) * inv;
+        store2<DT>(a.out, at + k * (HD / 8) + i, x, y);
       }
-    }
-  }
-  __syncthreads();
-  const int table_end = a.width << a.page_shift;
-  const int seq = max(a.seq_lens[b], 0);
-  const int p_first = seq - ql + r0 / grp, p_last = seq - ql + (r0 + nrows - 1) / grp;
-  const int lo_all = a.window ? max(p_first - a.window + 1, 0) : 0, hi_all = min(p_last + 1, table_end);
-  State<HD, PL> st;
-  float coef[R];
-  int row_lo[R], row_hi[R];
-  bool bad = seq > table_end;   // a length past the table: nan
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = g + 8 * r;
-    coef[r] = qexp[row] * (a.scale * 1.4426950408889634f);
-    const int p = seq - ql + (r0 + min(row, nrows - 1)) / grp;
-    row_lo[r] = a.window ? max(p - a.window + 1, 0) : 0;
-    row_hi[r] = p + 1;
-    st.m[r] = -INFINITY;
-    st.l[r] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) st.o[i][k] = 0.f;
-  const int bb = block_bytes(HD, a.group);
-  for (int blk = lo_all / kBlock + warp; blk * kBlock < hi_all; blk += kWarps) {
-    const int p0 = blk * kBlock;
-    const int page = a.table[b * a.table_stride + (p0 >> a.page_shift)];
-    if (page < 0 || page >= a.num_pages) {
-      bad = true;
-      continue;
-    }
-    const uint8_t* src = a.cache + ((((long)page * a.NKV + kvh) << (a.page_shift - 4)) +
-                                    ((p0 >> 4) & ((1 << (a.page_shift - 4)) - 1))) * bb;
-    const bool masked = p0 + kBlock > p_first + 1 || (a.window && p0 < p_last - a.window + 1);
-    int lo[R], hi[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      lo[r] = row_lo[r] - p0;
-      hi[r] = row_hi[r] - p0;
-    }
-    attend_block<HD, PL>(st, src, &qf[0][0], a.group, coef, masked, lo, hi, lo_all - p0, hi_all - p0);
-  }
-  // join the lanes of a row, then the warps
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
-    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
-    if (bad) st.l[r] = __int_as_float(0x7fc00000);
-    if (t == 0) {
-      red_m[warp][g + 8 * r] = st.m[r];
-      red_l[warp][g + 8 * r] = st.l[r];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int d = (2 * t + k) * (HD / 8) + i;
-      if (PL == 2) {
-        red_o[warp][g][d] = st.o[i][k] + st.o[i][k + 2];
-      } else {
-        red_o[warp][g][d] = st.o[i][k];
-        red_o[warp][ROWS - 8 + g][d] = st.o[i][k + 2];
-      }
-    }
-  __syncthreads();
-  for (int i = tid; i < nrows * HD; i += kThreads) {
-    const int r = i / HD, d = i - r * HD;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red_m[w][r]);
-    const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2f(red_m[w][r] - base);
-      l = fmaf(f, red_l[w][r], l);
-      o = fmaf(f, red_o[w][r][d], o);
-    }
-    const int row = r0 + r;
-    store_from_float(a.out, DT, ((long)(q0 + row / grp) * a.NH + kvh * grp + row % grp) * HD + d,
-                     l == 0.f ? 0.f : o / l);     // a row that sees nothing is zero
   }
 }
 
-// Rows of q past the last request are padding: zero.
-template <int DT>
-__global__ void kv4_padding_kernel(AttnArgs a, long row) {
-  const long used = (long)cu(a, a.B) * row;
-  for (long i = used + (long)blockIdx.x * blockDim.x + threadIdx.x; i < a.T * row; i += (long)gridDim.x * blockDim.x)
-    store_from_float(a.out, DT, i, 0.f);
+// The line of units cut for `warps` warps: the first `extra` of them take `each` + 1, the others `each`.
+struct Split {
+  long long warps, each, extra;
+  __device__ __forceinline__ Split() {}
+  __device__ __forceinline__ Split(long long units, int most) {
+    warps = min(units, (long long)most);
+    each = warps ? units / warps : 0;
+    extra = units - warps * each;
+  }
+  __device__ __forceinline__ long long start(long long w) const { return w * each + min(w, extra); }
+  __device__ __forceinline__ int warp_of(long long u) const {
+    const long long big = extra * (each + 1);
+    return (int)(u < big ? u / (each + 1) : extra + (u - big) / each);
+  }
+};
+
+// A warp's piece of the line and the tile it is at: in shared memory, since the loop over a tile's blocks
+// needs none of it and has no registers to spare.
+struct Piece {
+  long long u0, u1, u, us;      // the piece, the next tile in it, and where request b begins
+  long long item0, item1;       // the tile
+  Request r;
+  int b, kvh, r0, nrows, lo_all, hi_all;
+  int head, whole;              // its first tile began in an earlier warp; and goes on past this one
+};
+
+constexpr uint32_t kNoBlock = 0xffffffffu;
+
+// Block i of n from blk0 of request b, as its index in the cache; kNoBlock past the end or for a page
+// that is not one of the cache's.
+__device__ __forceinline__ uint32_t source(const AttnArgs& a, int b, int kvh, int blk0, int i, int n) {
+  const int shift = a.page_shift - 4;
+  if (i >= n) return kNoBlock;
+  const int page = a.table[b * a.table_stride + ((blk0 + i) >> shift)];
+  if (page < 0 || page >= a.num_pages) return kNoBlock;
+  return (((uint32_t)page * a.NKV + kvh) << shift) + ((blk0 + i) & ((1 << shift) - 1));
 }
 
-template <int DT, int HD>
-cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
+// A lane's block into a stage of the ring.
+template <int BB>
+__device__ __forceinline__ void issue(const AttnArgs& a, uint32_t src, int stage, uint32_t ring, uint32_t bar) {
+  if (src != kNoBlock) {
+    ptx::mbar_arrive_expect_tx(bar + 8 * stage, BB);
+    ptx::bulk_load(ring + stage * BB, a.cache + (size_t)src * BB, BB, bar + 8 * stage);
+  } else {
+    ptx::mbar_arrive(bar + 8 * stage);
+  }
+}
+
+struct Cross {          // a tile that this CTA shares with others
+  int valid, q0, kvh, r0, nrows, first, last, finish;
+};
+
+template <int DT, int HD, int G, int PL>
+__global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(AttnArgs a) {
+  constexpr int R = 3 - PL, ROWS = 16 / PL, NW = Shape<HD>::kWarps, ST = Shape<HD>::kStages, NT = Shape<HD>::kThreads;
+  constexpr int BB = block_bytes(HD, G);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long warp_sums[NW], start_unit[NW];
+  __shared__ int start_req[NW];
+  __shared__ Piece pieces[NW];
+  __shared__ Split sh_split;
+  __shared__ Cross cross[2];
+  __shared__ int abort_flag;
+  using L = Smem<HD, G>;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
   const int grp = a.NH / a.NKV;
+  uint8_t* ring = smem + L::kRing + warp * ST * BB;
+  uint4* qf = reinterpret_cast<uint4*>(smem + L::kQ) + warp * (HD / 16) * 32;
+  const uint32_t ring_s = ptx::smem_addr(ring), bar = ptx::smem_addr(smem + L::kBar) + warp * ST * 8;
+  if (lane == 0) {
+    for (int s = 0; s < ST; ++s) ptx::mbar_init(bar + 8 * s, 1);
+  }
+  if (tid == 0) {
+    abort_flag = 0;
+    cross[0].valid = cross[1].valid = 0;
+  }
+  ptx::fence_mbar_init();
+  __syncthreads();
+  // rows of no request are zero
+  const long used = (long)cu(a, a.B) * a.NH * HD, all = (long)a.T * a.NH * HD;
+  for (long i = used + (long)blockIdx.x * NT + tid; i < all; i += (long)gridDim.x * NT)
+    store_from_float(a.out, DT, i, 0.f);
+
+  // the line of units: where this warp's piece begins. Up to 32 requests each warp finds it alone;
+  // for more, every thread sums some requests and the block adds up.
+  const long long w0 = (long long)blockIdx.x * NW;
+  long long W = 0, us = 0;                     // units in all, and before request b
+  int b = 0;
+  Request r = {};
+  Split split;
+  if (a.B <= 32) {
+    if (lane < a.B) r = load_request<ROWS>(a, lane);
+    const long long mine = lane < a.B ? units_of(r, a.NKV) : 0;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    W = __shfl_sync(0xffffffffu, incl, 31);
+    split = Split(W, gridDim.x * NW);
+    if (w0 >= split.warps) return;
+    b = min(__popc(__ballot_sync(0xffffffffu, incl <= split.start(w0 + warp))), 31);
+    us = __shfl_sync(0xffffffffu, incl - mine, b);
+    r.q0 = __shfl_sync(0xffffffffu, r.q0, b);
+    r.ql = __shfl_sync(0xffffffffu, r.ql, b);
+    r.seq = __shfl_sync(0xffffffffu, r.seq, b);
+    r.tiles = __shfl_sync(0xffffffffu, r.tiles, b);
+    r.blo = __shfl_sync(0xffffffffu, r.blo, b);
+    r.nblk = __shfl_sync(0xffffffffu, r.nblk, b);
+  } else {
+    const int each = (a.B + NT - 1) / NT, b0 = min(tid * each, a.B), b1 = min(b0 + each, a.B);
+    long long mine = 0;
+    for (int i = b0; i < b1; ++i) mine += units_of(load_request<ROWS>(a, i), a.NKV);
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    long long before = incl - mine;
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) before += warp_sums[w];
+      W += warp_sums[w];
+    }
+    split = Split(W, gridDim.x * NW);
+    if (w0 >= split.warps) return;
+    if (mine > 0 && split.start(w0) < before + mine) {
+      long long s = before, n = 0;
+      int i = b0 - 1;
+      for (int w = 0; w < NW && w0 + w < split.warps; ++w) {
+        const long long u = split.start(w0 + w);
+        if (u < before) continue;
+        if (u >= before + mine) break;
+        while (i < b0 || u >= s + n) {
+          s += n;
+          n = units_of(load_request<ROWS>(a, ++i), a.NKV);
+        }
+        start_req[w] = i;
+        start_unit[w] = s;
+      }
+    }
+    __syncthreads();
+    if (w0 + warp < split.warps) {
+      b = start_req[warp];
+      us = start_unit[warp];
+      r = load_request<ROWS>(a, b);
+    }
+  }
+  const bool busy = w0 + warp < split.warps;
+  float* parts = a.parts + (long)blockIdx.x * (2 + NW) * Part<HD, PL>::kFloats;
+  Piece& c = pieces[warp];
+  if (lane == 0) {
+    c.r = r;
+    c.b = b;
+    c.us = us;
+    c.u0 = c.u = split.start(w0 + warp);
+    c.u1 = busy ? split.start(w0 + warp + 1) : c.u0;
+    c.item0 = c.item1 = 0;
+    c.head = c.whole = 0;
+    if (warp == 0) sh_split = split;
+  }
+  __syncwarp();
+  State<HD, PL> st;
+  int s = 0, phase = 0;                        // stage of the next block in the ring, and its parity
+  while (c.u < c.u1) {
+    // open the next tile of the piece
+    int blk0, n, first_masked, first_seen;
+    uint32_t src;
+    int pos[R];
+    float coef[R];
+    bool bad;
+    {
+      Request r = c.r;
+      int b = c.b;
+      long long us = c.us, u = c.u;
+      while (u >= us + units_of(r, a.NKV)) {
+        us += units_of(r, a.NKV);
+        r = load_request<ROWS>(a, ++b);
+      }
+      const int it = (int)((u - us) / r.nblk);
+      const long long item0 = us + (long long)it * r.nblk, item1 = item0 + r.nblk, end = min(item1, c.u1);
+      const int kvh = it / r.tiles, r0 = (it - kvh * r.tiles) * ROWS, nrows = min(ROWS, r.ql * grp - r0);
+      const int table_end = a.width << a.page_shift;
+      const int p_first = r.seq - r.ql + r0 / grp, p_last = r.seq - r.ql + (r0 + nrows - 1) / grp;
+      const int lo_all = a.window ? max(p_first - a.window + 1, 0) : 0, hi_all = min(p_last + 1, table_end);
+      // blocks of the piece that some row of the tile sees; all rows see those from first_seen to
+      // before first_masked
+      blk0 = max(r.blo + (int)(u - item0), lo_all / kBlock);
+      n = max(min(r.blo + (int)(end - item0), (hi_all + kBlock - 1) / kBlock) - blk0, 0);
+      first_masked = (p_first + 1) / kBlock - blk0;
+      first_seen = a.window ? (max(p_last - a.window + 1, 0) + kBlock - 1) / kBlock - blk0 : 0;
+      bad = r.seq > table_end;                  // a length past the table: nan
+#pragma unroll
+      for (int i = 0; i < R; ++i) pos[i] = r.seq - r.ql + (r0 + min(g + 8 * i, nrows - 1)) / grp;
+      __syncwarp();
+      if (lane == 0) {
+        c.r = r;
+        c.b = b;
+        c.us = us;
+        c.item0 = item0;
+        c.item1 = item1;
+        c.u = end;
+        c.kvh = kvh;
+        c.r0 = r0;
+        c.nrows = nrows;
+        c.lo_all = lo_all;
+        c.hi_all = hi_all;
+      }
+      src = source(a, b, kvh, blk0, lane, n);
+      load_queries<DT, HD, PL>(a, r, kvh, r0, nrows, grp, qf, coef, [&]() {
+        const int at = s + lane;
+        if (lane < min(ST, n)) issue<BB>(a, src, at < ST ? at : at - ST, ring_s, bar);
+      });
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      st.m[i] = -INFINITY;
+      st.l[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) st.o[i][j] = 0.f;
+    uint32_t next = kNoBlock, missing = 0;
+    __syncwarp();
+    for (int i = 0; i < n; ++i) {
+      if ((i & 31) == 0) {                        // lane j looks up block j of the 32 after these
+        missing = __ballot_sync(0xffffffffu, src == kNoBlock);
+        next = source(a, c.b, c.kvh, blk0, i + 32 + lane, n);
+      }
+      if (!ptx::mbar_wait(bar + 8 * s, phase, &abort_flag)) {
+        // gave up: nan for this tile, and no copy left in flight
+        bad = true;
+        for (int j = i; j < min(i + ST, n); ++j) {
+          ptx::mbar_wait_drain(bar + 8 * s, phase);
+          if (++s == ST) s = 0, phase ^= 1;
+        }
+        break;
+      }
+      if ((missing >> (i & 31)) & 1) {
+        bad = true;                               // a page that is not one of the cache's: nan
+      } else if (i >= first_seen && i < first_masked) {
+        const int all[R] = {};
+        attend_block<HD, G, PL, false>(st, ring + s * BB, qf, coef, all, all, 0, kBlock);
+      } else {
+        const int p0 = (blk0 + i) * kBlock;
+        int lo[R], hi[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          lo[j] = (a.window ? max(pos[j] - a.window + 1, 0) : 0) - p0;
+          hi[j] = pos[j] + 1 - p0;
+        }
+        attend_block<HD, G, PL, true>(st, ring + s * BB, qf, coef, lo, hi, c.lo_all - p0, c.hi_all - p0);
+      }
+      __syncwarp();
+      const int ahead = i + ST;                  // the stage is free: block i + ST goes there
+      if (ahead < n && (ahead & 31) == lane) issue<BB>(a, (ahead ^ i) & 32 ? next : src, s, ring_s, bar);
+      if ((i & 31) == 31) src = next;
+      if (++s == ST) s = 0, phase ^= 1;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 1);
+      st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 2);
+      if (bad) st.l[i] = __int_as_float(0x7fc00000);
+    }
+    if (c.item0 >= c.u0 && c.item1 <= c.u1) {
+      write_tile<DT, HD, PL>(a, st, c.r.q0, c.kvh, c.r0, c.nrows, grp);
+    } else if (c.item0 < c.u0) {                 // began in an earlier warp
+      if (c.u < c.u1) store_part<HD, PL>(st, parts + (2 + warp) * Part<HD, PL>::kFloats);
+      if (lane == 0) {
+        c.head = 1;
+        c.whole = c.item1 > c.u1;
+        if (warp == 0)
+          cross[0] = {1, c.r.q0, c.kvh, c.r0, c.nrows, sh_split.warp_of(c.item0) / NW, sh_split.warp_of(c.item1 - 1) / NW, 0};
+      }
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+
+  // join the parts of this CTA's warps: a tile's parts are in consecutive warps, and the warp where it
+  // begins (warp 0 for one that began in another CTA) takes the others in their order. The parts move
+  // to shared memory, where the rings and queries are done with.
+  constexpr int SIZE = Part<HD, PL>::kFloats;
+  float* shared_parts = reinterpret_cast<float*>(smem);
+  static_assert(NW * SIZE * 4 <= L::kBar, "the parts of a CTA's warps fit where its rings were");
+  const bool last_is_head = c.item0 < c.u0 && c.head;
+  if (c.head && warp > 0) {
+    if (last_is_head) {
+      store_part<HD, PL>(st, shared_parts + warp * SIZE);
+    } else {
+      copy_part<HD, PL>(shared_parts + warp * SIZE, parts + (2 + warp) * SIZE);
+    }
+  }
+  __syncthreads();
+  // parts that follow this warp's, and whether the tile ends with them
+  const auto following = [&](bool& open) {
+    int n = 0;
+    for (int w = warp + 1; open && w < NW && pieces[w].head; ++w) {
+      ++n;
+      open = pieces[w].whole;
+    }
+    return n;
+  };
+  if (warp == 0 && c.head) {
+    if (last_is_head) {
+      bool open = c.whole;
+      const int n = following(open);
+      join_parts<HD, PL>(st, shared_parts + SIZE, n);
+      store_part<HD, PL>(st, parts);
+    } else {                                     // its state went on to another tile: the part is as it was
+      copy_part<HD, PL>(parts, parts + 2 * SIZE);
+    }
+  }
+  if (c.item1 > c.u1 && c.item0 >= c.u0) {       // a tile that begins here and goes on
+    bool open = true;
+    const int n = following(open);
+    join_parts<HD, PL>(st, shared_parts + (warp + 1) * SIZE, n);
+    if (!open) {
+      write_tile<DT, HD, PL>(a, st, c.r.q0, c.kvh, c.r0, c.nrows, grp);
+    } else {
+      if (lane == 0)
+        cross[1] = {1, c.r.q0, c.kvh, c.r0, c.nrows, (int)blockIdx.x, sh_split.warp_of(c.item1 - 1) / NW, 0};
+      store_part<HD, PL>(st, parts + SIZE);
+    }
+  }
+  if (tid == 0 && abort_flag) atomicExch(&g_kv4_status, 1);
+  __threadfence();
+  __syncthreads();
+  if (tid < 2 && cross[tid].valid) {
+    // of the CTAs that share the tile, the last to arrive joins their parts
+    const Cross x = cross[tid];
+    const bool done = atomicAdd(&a.counters[x.first], 1u) == (unsigned)(x.last - x.first);
+    if (done) a.counters[x.first] = 0u;
+    cross[tid].finish = done;
+  }
+  __syncthreads();
+  float* weight = reinterpret_cast<float*>(smem);   // [parts][16], in the ring, which is idle now
+  for (int k = 0; k < 2; ++k) {
+    const Cross x = cross[k];
+    if (!x.valid || !x.finish) continue;
+    __threadfence();
+    const int n = x.last - x.first + 1;
+    const auto part_of = [&](int p) {
+      return a.parts + ((long)(x.first + p) * (2 + NW) + (p == 0 ? 1 : 0)) * SIZE;
+    };
+    float* top = weight + n * 16;                // the parts' m, then l
+    for (int i = tid; i < n * 16; i += NT) {
+      const float* ml = part_of(i >> 4) + Part<HD, PL>::kStats + (i & 15);
+      top[i] = __ldcg(ml);
+      top[n * 16 + i] = __ldcg(ml + 16);
+    }
+    __syncthreads();
+    for (int row = warp; row < ROWS; row += NW) {
+      float m = -INFINITY, l = 0.f;
+      for (int p = lane; p < n; p += 32) m = fmaxf(m, top[p * 16 + row]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float base = m == -INFINITY ? 0.f : m;
+      for (int p = lane; p < n; p += 32) l = fmaf(ex2(top[p * 16 + row] - base), top[(n + p) * 16 + row], l);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      for (int p = lane; p < n; p += 32) weight[p * 16 + row] = ex2(top[p * 16 + row] - base) * inv;
+    }
+    __syncthreads();
+    // four floats a thread: two neighbouring lanes of a fragment, or one lane's two rows
+    for (int i = tid; i < HD / 8 * 32 / PL; i += NT) {
+      const int ln = i * PL & 31, gg = ln >> 2, tile = i * PL >> 5;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 16
+      for (int p = 0; p < n; ++p) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(p)) + i);
+        const float f0 = weight[p * 16 + gg], f1 = PL == 2 ? f0 : weight[p * 16 + 8 + gg];
+        acc.x = fmaf(f0, v.x, acc.x);
+        acc.y = fmaf(f0, v.y, acc.y);
+        acc.z = fmaf(f1, v.z, acc.z);
+        acc.w = fmaf(f1, v.w, acc.w);
+      }
+      // lane (g, t) of tile i: elements 2t HD / 8 + i and HD / 8 past it
+      const int e = 2 * (ln & 3) * (HD / 8) + tile;
+      const float out[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = PL == 2 ? gg : gg + 8 * h, at = PL == 2 ? e + 2 * h * (HD / 8) : e;
+        if (row < x.nrows) {
+          const long o = out_row(a, x.q0, x.kvh, x.r0 + row, grp) * HD + at;
+          store_from_float(a.out, DT, o, out[2 * h]);
+          store_from_float(a.out, DT, o + HD / 8, out[2 * h + 1]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+int sm_count() {
+  int sms = 148, dev = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms <= 0 ? 148 : sms < kMaxCtas ? sms : kMaxCtas;
+}
+
+template <int HD>
+constexpr size_t part_floats() {
+  return (size_t)(2 + Shape<HD>::kWarps) * (HD == 256 ? Part<HD, 2>::kFloats : Part<HD, 1>::kFloats);
+}
+size_t parts_bytes(int HD, int ctas) {
+  return (HD == 64 ? part_floats<64>() : HD == 128 ? part_floats<128>() : part_floats<256>()) * ctas * sizeof(float);
+}
+
+template <int DT, int HD, int G, int PL>
+int launch_one(const AttnArgs& a, int ctas, cudaStream_t st) {
+  auto kern = kv4_attention_kernel<DT, HD, G, PL>;
+  static int configured_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_dev != dev) {
+    const int rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, G>::kBytes),
+                               "cudaFuncSetAttribute(kv4 attention smem)");
+    if (rc) return rc;
+    configured_dev = dev;
+  }
+  kern<<<ctas, Shape<HD>::kThreads, Smem<HD, G>::kBytes, st>>>(a);
+  return cuda_status(cudaGetLastError(), "ql_kv4_attention launch");
+}
+
+template <int DT, int HD, int G>
+int launch(const AttnArgs& a, int ctas, cudaStream_t st) {
   // one plane where 16-bit inputs fill more than 8 rows: their outputs keep no more than the 11 bits
   // of a single fp16 probability (HD = 256 has no registers for 16 rows)
-  constexpr bool can = DT != QL_F32 && HD != 256;
-  const bool one_plane = can && (long)a.T * grp > 8L * a.B;
-  const int rows = one_plane ? 16 : 8;
-  const dim3 grid((unsigned)((long)a.T * grp / rows + a.B), a.NKV);
-  if (one_plane) kv4_attention_kernel<DT, HD, (can ? 1 : 2)><<<grid, kThreads, 0, st>>>(a);
-  else kv4_attention_kernel<DT, HD, 2><<<grid, kThreads, 0, st>>>(a);
-  if (a.cu_q || a.T > a.B) kv4_padding_kernel<DT><<<64, 256, 0, st>>>(a, (long)a.NH * HD);
-  return cudaGetLastError();
+  constexpr bool can = HD != 256 && DT != QL_F32;
+  if (can && (long)a.T * (a.NH / a.NKV) > 8L * a.B) return launch_one<DT, HD, G, can ? 1 : 2>(a, ctas, st);
+  return launch_one<DT, HD, G, 2>(a, ctas, st);
 }
 
 template <int DT>
-cudaError_t launch_hd(const AttnArgs& a, int HD, cudaStream_t st) {
-  return HD == 64 ? launch<DT, 64>(a, st) : HD == 128 ? launch<DT, 128>(a, st) : launch<DT, 256>(a, st);
+int launch_sizes(const AttnArgs& a, int HD, int group, int ctas, cudaStream_t st) {
+  if (HD == 64) return group == 32 ? launch<DT, 64, 32>(a, ctas, st) : launch<DT, 64, 64>(a, ctas, st);
+  if (HD == 128)
+    return group == 32   ? launch<DT, 128, 32>(a, ctas, st)
+           : group == 64 ? launch<DT, 128, 64>(a, ctas, st)
+                         : launch<DT, 128, 128>(a, ctas, st);
+  return group == 32   ? launch<DT, 256, 32>(a, ctas, st)
+         : group == 64 ? launch<DT, 256, 64>(a, ctas, st)
+                       : launch<DT, 256, 128>(a, ctas, st);
 }
 
 }  // namespace
+
+int take_kv4_status() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_kv4_status, sizeof(int)) != cudaSuccess) return 0;
+  if (v) cudaMemcpyToSymbol(g_kv4_status, &zero, sizeof(int));
+  return v;
+}
+
 }  // namespace ql
 
 using namespace ql;
 
 extern "C" size_t ql_kv4_attention_workspace(int NH, int NKV, int HD) {
-  (void)NH;
-  (void)NKV;
-  (void)HD;
-  return 0;
+  if (!kv4::sizes_ok(NKV, HD, 16, 32) || NH <= 0) return 0;
+  return kMaxCtas * sizeof(unsigned int) + parts_bytes(HD, sm_count());
 }
 
 extern "C" int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int NH, int NKV, int HD, const void* cache,
@@ -410,9 +956,19 @@ extern "C" int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int N
     return QL_ERR_ARG;
   }
   const size_t need = ql_kv4_attention_workspace(NH, NKV, HD);
-  if (need && (!workspace || workspace_bytes < need)) {
-    set_error("ql_kv4_attention: workspace of %zu bytes needed", need);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)) {
+    set_error("ql_kv4_attention: workspace of %zu bytes (16-byte aligned, zeroed once) needed", need);
     return QL_ERR_ARG;
+  }
+  if ((long)num_pages * NKV * (page / kv4::kBlock) >= 0xffffffffl) {
+    set_error("ql_kv4_attention: a cache of %ld blocks is past 32 bits", (long)num_pages * NKV * (page / kv4::kBlock));
+    return QL_ERR_UNSUPPORTED;
+  }
+  const int ctas = sm_count();
+  const size_t es = dtype == QL_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(out) % 8 || reinterpret_cast<uintptr_t>(q) % 16 || ldq * es % 16) {
+    set_error("ql_kv4_attention: out must be 8-byte aligned, the tokens of q 16-byte aligned (ldq=%ld)", ldq);
+    return QL_ERR_ALIGN;
   }
   AttnArgs a;
   a.q = q;
@@ -423,7 +979,6 @@ extern "C" int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int N
   a.cache = reinterpret_cast<const uint8_t*>(cache);
   a.num_pages = num_pages;
   a.page_shift = __builtin_ctz((unsigned)page);
-  a.group = group;
   a.table = table;
   a.table_stride = table_stride;
   a.width = table_width;
@@ -433,8 +988,10 @@ extern "C" int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int N
   a.scale = scale;
   a.window = window;
   a.out = out;
+  a.counters = reinterpret_cast<unsigned int*>(workspace);
+  a.parts = reinterpret_cast<float*>(a.counters + kMaxCtas);
   const cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = dtype == QL_F32 ? launch_hd<QL_F32>(a, HD, st)
-                        : dtype == QL_F16 ? launch_hd<QL_F16>(a, HD, st) : launch_hd<QL_BF16>(a, HD, st);
-  return cuda_status(e, "ql_kv4_attention launch");
+  return dtype == QL_F32   ? launch_sizes<QL_F32>(a, HD, group, ctas, st)
+         : dtype == QL_F16 ? launch_sizes<QL_F16>(a, HD, group, ctas, st)
+                           : launch_sizes<QL_BF16>(a, HD, group, ctas, st);
 }

@@ -57,7 +57,6 @@ class KV4Cache:
         self.data = data
         self.num_pages, self.NKV, self.HD, self.page, self.group = num_pages, NKV, HD, page, group
         self.device = data.device
-        self._ws = {}
 
     def nbytes(self):
         return self.data.numel()
@@ -72,19 +71,23 @@ class KV4Cache:
                   slots.data_ptr(), T, k.data_ptr(), v.data_ptr(), _ffi.stream_ptr(stream, self.device))
         return k, v
 
-    def _workspace(self, NH, stream):
-        """The attention's workspace on this stream, made once: its counters are zero between calls, and
-        calls that share one may not overlap."""
-        key = (NH, _ffi.stream_ptr(stream, self.device))
-        ws = self._ws.get(key)
-        if ws is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("attention needs its workspace before a graph is captured: call it once on this "
-                                   "stream first, or pass workspace=")
-            n = int(_ffi.fn("ql_kv4_attention_workspace")(NH, self.NKV, self.HD))
-            with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(self.device)):
-                ws = self._ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
-        return ws
+
+_workspaces = {}
+
+
+def _attention_workspace(cache, NH, stream):
+    """The attention's workspace on this stream, made once and shared by the layers' caches: its counters
+    are zero between calls, and calls that share one may not overlap."""
+    key = (cache.device, cache.HD, _ffi.stream_ptr(stream, cache.device))
+    ws = _workspaces.get(key)
+    if ws is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("attention needs its workspace before a graph is captured: call it once on this "
+                               "stream first, or pass workspace=")
+        n = int(_ffi.fn("ql_kv4_attention_workspace")(NH, cache.NKV, cache.HD))
+        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(cache.device)):
+            ws = _workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=cache.device)
+    return ws
 
 
 def plan(prev_lens, new_lens, block_table, free_pages, n_free, page, max_tokens, stream=None):
@@ -165,7 +168,9 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
     q [T, NH, HD] fp32, fp16 or bf16 (heads contiguous; tokens may be strided): rows cu_q[b] ..
     cu_q[b + 1] - 1 are request b's last tokens (cu_q int32 [B + 1]; None: one token each). block_table
     int32 [B, width], seq_lens int32 [B] with those tokens counted. window: positions that a query sees
-    (0: all). Rows that see nothing, and rows past cu_q[B], are zero. Returns [T, NH, HD] in q's dtype."""
+    (0: all). workspace: uint8 of ql_kv4_attention_workspace bytes, zeroed once and not shared by calls that
+    overlap (None: one for each stream). Rows that see nothing, and rows past cu_q[B], are zero. Returns
+    [T, NH, HD] in q's dtype."""
     if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
         raise ValueError("q must be [T, NH, HD] with contiguous heads, got %s" % (tuple(q.shape),))
     _need(q, "q", q.dtype, 3)
@@ -183,12 +188,15 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
         _need(cu_q, "cu_q", torch.int32, 1)
         if cu_q.shape[0] != B + 1:
             raise ValueError("cu_q must be [%d]" % (B + 1))
+    ldq = q.stride(0) if T > 1 else NH * HD
+    if q.data_ptr() % 16 or ldq * q.element_size() % 16:      # the kernel reads 16 bytes at a time
+        q, ldq = torch.empty((T, NH, HD), dtype=q.dtype, device=q.device).copy_(q), NH * HD
     if out is None:
         out = torch.empty((T, NH, HD), dtype=q.dtype, device=q.device)
     elif out.dtype != q.dtype or tuple(out.shape) != (T, NH, HD) or not out.is_contiguous():
         raise ValueError("out must be a contiguous %s tensor %s" % (q.dtype, (T, NH, HD)))
-    ws = cache._workspace(NH, stream) if workspace is None else workspace
-    _ffi.call("ql_kv4_attention", q.data_ptr(), _ffi.dtype_code(q.dtype), max(q.stride(0), NH * HD), T, NH, cache.NKV, HD,
+    ws = _attention_workspace(cache, NH, stream) if workspace is None else workspace
+    _ffi.call("ql_kv4_attention", q.data_ptr(), _ffi.dtype_code(q.dtype), ldq, T, NH, cache.NKV, HD,
               cache.data.data_ptr(), cache.num_pages, cache.page, cache.group, block_table.data_ptr(),
               max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], seq_lens.data_ptr(), _ffi.ptr(cu_q),
               B, float(scale) if scale is not None else 1.0 / math.sqrt(HD), int(window), out.data_ptr(), ws.data_ptr(),
