@@ -30,7 +30,7 @@ def _plan(lib, **kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(n=0), 1), (dict(page=8), 1), (dict(page=24), 1), (dict(page=8192), 1), (dict(stride=4), 1), (dict(width=0), 1),
     (dict(cap=0), 1), (dict(max_tokens=-1), 1), (dict(slots=0), 1), (dict(prev=0), 1), (dict(lens=16), 1),
-    (dict(left=256), 1), (dict(ws=0), 1), (dict(ws_bytes=8), 1), (dict(width=1 << 20, stride=1 << 20, page=4096), 3),
+    (dict(left=256), 1), (dict(n=20000, ws=0), 1), (dict(n=20000, ws_bytes=8), 1), (dict(width=1 << 20, stride=1 << 20, page=4096), 3),
 ])
 def test_plan_refuses(lib, kw, code):
     assert _plan(lib, **kw) == code

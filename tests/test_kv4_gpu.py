@@ -66,7 +66,7 @@ def make_plan(n, longest, page, spare, seed, ended=0.1, prompts=0.2, width_extra
 
 @pytest.mark.parametrize("n,longest,page,spare,cap", [
     (1, 40, 16, 3, 64), (1, 0, 16, 1, 0), (7, 100, 16, 40, 400), (33, 500, 32, 5, 300), (256, 60, 16, 1000, 20000),
-    (1024, 90, 64, 200, 5000), (1025, 33, 16, 2000, 30000), (2500, 300, 128, 700, 100000), (5000, 200, 16, 30000, 1 << 19),
+    (1024, 90, 64, 200, 5000), (1025, 33, 16, 2000, 30000), (2500, 300, 128, 700, 100000), (5000, 200, 16, 30000, 1 << 19), (16385, 40, 16, 30000, 100000), (40000, 20, 16, 20000, 9000),
 ])
 def test_plan(n, longest, page, spare, cap):
     check_plan(*make_plan(n, longest, page, spare, n), page, cap)

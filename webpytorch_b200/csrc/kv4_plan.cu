@@ -11,8 +11,8 @@
 namespace ql {
 namespace {
 
-constexpr int kScanThreads = 1024;
-constexpr int kFillThreads = 256;
+constexpr int kThreads = 1024;
+constexpr int kMost = 16384;   // requests whose sums fit in shared memory
 
 struct PlanArgs {
   const int32_t* prev;
@@ -30,13 +30,13 @@ struct PlanArgs {
   int32_t* positions;
   int32_t* requests;
   int32_t* n_free_out;
-  int32_t* need_end;   // [n] workspace: inclusive sums of pages taken
-  int32_t* back_end;   // [n] workspace: inclusive sums of pages given back
-  int32_t* totals;     // [2] workspace: avail, pages taken
+  int32_t* sums;          // workspace for more than kMost requests: three arrays of n + 1
 };
 
 struct Request {
-  long long back, need, tok;
+  int back, need;
+  long long tok;
+  int len;
   bool fits, over;
 };
 
@@ -45,10 +45,10 @@ __device__ __forceinline__ int pages_of(long long len, int shift) {
 }
 
 __device__ __forceinline__ Request load_request(const PlanArgs& a, int b) {
-  Request r = {0, 0, 0, false, false};
-  if (b >= a.n) return r;
+  Request r = {};
   const long long prev = max(a.prev[b], 0);
   const long long fresh = a.fresh[b];
+  r.len = (int)prev;
   const int held = pages_of(prev, a.page_shift);
   r.over = fresh < 0;
   if (r.over) {
@@ -64,64 +64,36 @@ __device__ __forceinline__ Request load_request(const PlanArgs& a, int b) {
   return r;
 }
 
-// Inclusive sum over the block; *total receives the block's sum.
-__device__ __forceinline__ long long block_scan(long long v, long long* warps, long long* total) {
+// Sums over the threads before this one, and over all of them.
+template <int N>
+__device__ __forceinline__ void block_scan(long long (&v)[N], long long (&total)[N], long long (*warps)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long incl[N];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
-  __syncthreads();
-  if (lane == 31) warps[warp] = v;
-  __syncthreads();
-  long long before = 0, all = 0;
-  for (int w = 0; w < kScanThreads / 32; ++w) {
-    const long long x = warps[w];
-    if (w < warp) before += x;
-    all += x;
-  }
-  *total = all;
-  return v + before;
-}
-
-__global__ void __launch_bounds__(kScanThreads) plan_scan_kernel(PlanArgs a) {
-  __shared__ long long warps[kScanThreads / 32];
-  const int tid = threadIdx.x;
-  long long total, back_all = 0;
-  for (int b0 = 0; b0 < a.n; b0 += kScanThreads) {
-    const Request r = load_request(a, b0 + tid);
-    const long long end = back_all + block_scan(r.back, warps, &total);
-    if (b0 + tid < a.n) a.back_end[b0 + tid] = (int32_t)min(end, (long long)INT32_MAX);
-    back_all += total;
-  }
-  const long long n_free = min(max(*a.n_free_in, 0), a.free_capacity);
-  const long long avail = min(n_free + back_all, (long long)a.free_capacity);
-  long long need0 = 0, tok0 = 0, put0 = 0, taken = 0;
-  for (int b0 = 0; b0 < a.n; b0 += kScanThreads) {
-    const int b = b0 + tid;
-    const Request r = load_request(a, b);
-    const long long need_end = need0 + block_scan(r.need, warps, &total);
-    need0 += total;
-    const long long tok_end = tok0 + block_scan(r.tok, warps, &total);
-    tok0 += total;
-    const bool served = r.fits && tok_end <= a.max_tokens && (r.need == 0 || need_end <= avail);
-    const long long put = served ? r.tok : 0;
-    const long long put_end = put0 + block_scan(put, warps, &total);
-    put0 += total;
-    const long long taken_end = taken + block_scan(served ? r.need : 0, warps, &total);
-    taken += total;
-    if (b < a.n) {
-      a.cu_new[b] = (int32_t)(put_end - put);
-      a.seq_lens[b] = r.over ? 0 : max(a.prev[b], 0) + (int32_t)put;
-      a.need_end[b] = (int32_t)taken_end;
+  for (int k = 0; k < N; ++k) {
+    incl[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, incl[k], o);
+      if (lane >= o) incl[k] += u;
     }
   }
-  if (tid == 0) {
-    a.cu_new[a.n] = (int32_t)put0;
-    a.n_free_out[0] = (int32_t)(avail - taken);
-    a.totals[0] = (int32_t)avail;
-    a.totals[1] = (int32_t)taken;
+  __syncthreads();
+  if (lane == 31)
+#pragma unroll
+    for (int k = 0; k < N; ++k) warps[warp][k] = incl[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const long long own = warps[lane][k];      // kThreads / 32 = 32 warps
+    long long all = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, all, o);
+      if (lane >= o) all += u;
+    }
+    total[k] = __shfl_sync(0xffffffffu, all, 31);
+    v[k] = incl[k] - v[k] + __shfl_sync(0xffffffffu, all - own, warp);
   }
 }
 
@@ -138,29 +110,90 @@ __device__ __forceinline__ int find(const int32_t* end, int n, int i) {
 
 // Entry i of the stack of free pages after the returned ones are pushed. The pushes are made by
 // other threads of the same launch, so entries above the old top come from the rows they leave.
-__device__ __forceinline__ int32_t stack_entry(const PlanArgs& a, int n_free, int i) {
+__device__ __forceinline__ int32_t stack_entry(const PlanArgs& a, const int32_t* back_end, int n_free, int i) {
   if (i < n_free) return a.free_pages[i];
   const int k = i - n_free;
-  const int b = find(a.back_end, a.n, k);
-  return a.table[b * a.table_stride + k - (b ? a.back_end[b - 1] : 0)];
+  const int b = find(back_end, a.n, k);
+  return a.table[b * a.table_stride + k - (b ? back_end[b - 1] : 0)];
 }
 
-__global__ void __launch_bounds__(kFillThreads) plan_fill_kernel(PlanArgs a) {
-  const int t0 = blockIdx.x * kFillThreads + threadIdx.x, step = gridDim.x * kFillThreads;
+// Every CTA sums over all requests (8 bytes a request from L2, two block scans), so that one launch does
+// without any exchange between CTAs, then writes its share of the tokens and pages. SHARED: the sums are in
+// its shared memory, where the binary searches run; for more requests than fit, in a workspace that every
+// CTA fills alike.
+template <bool SHARED>
+__global__ void __launch_bounds__(kThreads) plan_kernel(PlanArgs a) {
+  extern __shared__ int32_t shared_sums[];
+  __shared__ long long warps3[kThreads / 32][3], warps2[kThreads / 32][2];
+  int32_t* cu = SHARED ? shared_sums : a.sums + (long)blockIdx.x * 3 * (a.n + 1);
+  int32_t* need_end = cu + a.n + 1;       // inclusive sums of pages taken
+  int32_t* back_end = need_end + a.n;     // and of pages given back
+  const int tid = threadIdx.x;
+  const int each = (a.n + kThreads - 1) / kThreads, b0 = min(tid * each, a.n), b1 = min(b0 + each, a.n);
+  long long v[3] = {}, all[3];
+  for (int b = b0; b < b1; ++b) {
+    const Request r = load_request(a, b);
+    v[0] += r.back;
+    v[1] += r.need;
+    v[2] += r.tok;
+  }
+  block_scan<3>(v, all, warps3);
   const int n_free = min(max(*a.n_free_in, 0), a.free_capacity);
-  const int avail = a.totals[0], taken = a.totals[1], total = a.cu_new[a.n];
-  const int page = 1 << a.page_shift;
+  const int avail = (int)min(n_free + all[0], (long long)a.free_capacity);
+  long long w[2] = {}, sums[2];
+  {
+    long long need = v[1], tok = v[2];
+    for (int b = b0; b < b1; ++b) {
+      const Request r = load_request(a, b);
+      need += r.need;
+      tok += r.tok;
+      if (r.fits && tok <= a.max_tokens && (r.need == 0 || need <= avail)) {
+        w[0] += r.tok;
+        w[1] += r.need;
+      }
+    }
+  }
+  block_scan<2>(w, sums, warps2);
+  const int total = (int)sums[0], taken = (int)sums[1];
+  for (int b = b0; b < b1; ++b) {
+    const Request r = load_request(a, b);
+    v[0] += r.back;
+    v[1] += r.need;
+    v[2] += r.tok;
+    const bool served = r.fits && v[2] <= a.max_tokens && (r.need == 0 || v[1] <= avail);
+    cu[b] = (int32_t)w[0];
+    if (blockIdx.x == 0) {
+      a.cu_new[b] = (int32_t)w[0];
+      a.seq_lens[b] = r.over ? 0 : r.len + (served ? (int)r.tok : 0);
+    }
+    if (served) {
+      w[0] += r.tok;
+      w[1] += r.need;
+    }
+    need_end[b] = (int32_t)w[1];
+    back_end[b] = (int32_t)v[0];
+  }
+  if (tid == 0) {
+    cu[a.n] = total;
+    if (blockIdx.x == 0) {
+      a.cu_new[a.n] = total;
+      a.n_free_out[0] = avail - taken;
+    }
+  }
+  __syncthreads();
+
+  const int t0 = blockIdx.x * kThreads + tid, step = gridDim.x * kThreads, page = 1 << a.page_shift;
   for (int t = t0; t < a.max_tokens; t += step) {
     int64_t slot = -1;
     int pos = -1, b = -1;
     if (t < total) {
-      b = find(a.cu_new + 1, a.n, t);
+      b = find(cu + 1, a.n, t);
       const int prev = max(a.prev[b], 0);
       const int held = pages_of(prev, a.page_shift);
-      pos = prev + t - a.cu_new[b];
+      pos = prev + t - cu[b];
       const int i = pos >> a.page_shift;
       const int32_t p = i < held ? a.table[b * a.table_stride + i]
-                                 : stack_entry(a, n_free, avail - 1 - ((b ? a.need_end[b - 1] : 0) + i - held));
+                                 : stack_entry(a, back_end, n_free, avail - 1 - ((b ? need_end[b - 1] : 0) + i - held));
       slot = (int64_t)p * page + (pos & (page - 1));
     }
     a.slots[t] = slot;
@@ -168,12 +201,16 @@ __global__ void __launch_bounds__(kFillThreads) plan_fill_kernel(PlanArgs a) {
     a.requests[t] = b;
   }
   for (int k = t0; k < taken; k += step) {   // pages taken: table entries past the held ones
-    const int b = find(a.need_end, a.n, k);
+    const int b = find(need_end, a.n, k);
     const int held = pages_of(max(a.prev[b], 0), a.page_shift);
-    a.table[b * a.table_stride + held + k - (b ? a.need_end[b - 1] : 0)] = stack_entry(a, n_free, avail - 1 - k);
+    a.table[b * a.table_stride + held + k - (b ? need_end[b - 1] : 0)] = stack_entry(a, back_end, n_free, avail - 1 - k);
   }
   for (int k = n_free + t0; k < avail; k += step)   // pages given back
-    a.free_pages[k] = stack_entry(a, n_free, k);
+    a.free_pages[k] = stack_entry(a, back_end, n_free, k);
+}
+
+int ctas_for(int n, int max_tokens) {
+  return max(1, min(n <= kMost ? 148 : 16, (max(max_tokens, n) + kThreads - 1) / kThreads));
 }
 
 }  // namespace
@@ -181,7 +218,9 @@ __global__ void __launch_bounds__(kFillThreads) plan_fill_kernel(PlanArgs a) {
 
 using namespace ql;
 
-extern "C" size_t ql_kv_plan_workspace(int n) { return n <= 0 ? 0 : ((size_t)2 * n + 2) * sizeof(int32_t); }
+extern "C" size_t ql_kv_plan_workspace(int n) {
+  return n <= kMost ? 0 : (size_t)16 * 3 * (n + 1) * sizeof(int32_t);
+}
 
 extern "C" int ql_kv_plan(const int32_t* prev_lens, const int32_t* new_lens, int n, int32_t* table, long table_stride,
                           int table_width, int32_t* free_pages, int free_capacity, const int32_t* n_free, int page,
@@ -203,7 +242,7 @@ extern "C" int ql_kv_plan(const int32_t* prev_lens, const int32_t* new_lens, int
     set_error("ql_kv_plan: seq_lens and n_free_out may not be prev_lens and n_free");
     return QL_ERR_ARG;
   }
-  if (!workspace || workspace_bytes < ql_kv_plan_workspace(n)) {
+  if (ql_kv_plan_workspace(n) > 0 && (!workspace || workspace_bytes < ql_kv_plan_workspace(n))) {
     set_error("ql_kv_plan: workspace of %zu bytes needed", ql_kv_plan_workspace(n));
     return QL_ERR_ARG;
   }
@@ -225,12 +264,23 @@ extern "C" int ql_kv_plan(const int32_t* prev_lens, const int32_t* new_lens, int
   a.positions = positions;
   a.requests = requests;
   a.n_free_out = n_free_out;
-  a.need_end = reinterpret_cast<int32_t*>(workspace);
-  a.back_end = a.need_end + n;
-  a.totals = a.back_end + n;
+  a.sums = reinterpret_cast<int32_t*>(workspace);
   const cudaStream_t st = (cudaStream_t)stream;
-  plan_scan_kernel<<<1, kScanThreads, 0, st>>>(a);
-  const int blocks = max(1, min(148 * 8, (max(max_tokens, n) + kFillThreads - 1) / kFillThreads));
-  plan_fill_kernel<<<blocks, kFillThreads, 0, st>>>(a);
+  const int ctas = ctas_for(n, max_tokens);
+  if (n > kMost) {
+    plan_kernel<false><<<ctas, kThreads, 0, st>>>(a);
+  } else {
+    static int configured_dev = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (configured_dev != dev) {
+      const int rc = cuda_status(cudaFuncSetAttribute(plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                      3 * (kMost + 1) * (int)sizeof(int32_t)),
+                                 "cudaFuncSetAttribute(plan smem)");
+      if (rc) return rc;
+      configured_dev = dev;
+    }
+    plan_kernel<true><<<ctas, kThreads, 3 * (size_t)(n + 1) * sizeof(int32_t), st>>>(a);
+  }
   return cuda_status(cudaGetLastError(), "ql_kv_plan launch");
 }

@@ -48,7 +48,7 @@ __device__ __forceinline__ uint8_t* block_of(const RopeArgs& a, long slot, int g
          (long)(r >> 4) * block_bytes(HD, a.group);
 }
 
-// One warp per (token, head); lane l holds elements V l .. V l + V - 1.
+// Any row alignment and any rot: one warp per (token, head), lane l holds elements V l .. V l + V - 1.
 template <int DT, int HD>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
   constexpr int V = HD / 32;
@@ -142,31 +142,218 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
     reinterpret_cast<__half2*>(blk + code_bytes(HD))[r * (HD / a.group) + lane / gl] = __halves2half2(s, m);
 }
 
-// The values that slots stand for: one warp per (token, head).
-template <int HD>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(RopeArgs a, __half* k_out, __half* v_out) {
-  constexpr int V = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const long item = (long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (item >= (long)a.T * 2 * a.NKV) return;
-  const long t = item / (2 * a.NKV);
-  const int h = (int)(item - t * 2 * a.NKV), g = h % a.NKV;
-  const bool is_v = h >= a.NKV;
-  const long slot = a.slots[t];
-  __half* out = (is_v ? v_out : k_out) + (t * a.NKV + g) * HD + lane * V;
-  if (slot < 0 || slot >= a.num_slots) {
+// Rows of 16-byte aligned heads whose rotated halves are whole 16-byte pieces: a lane holds E consecutive
+// elements (16 bytes; 8 fp32 elements at HD = 256), so 16 bytes a lane are read and written, a warp takes 32 E / HD
+// heads at a time, and one token's cos, sin and slot serve all of its heads. `split` warps share a token, so that
+// few tokens still fill the GPU. kAhead loads are under way at once.
+constexpr int kVecThreads = 256;
+constexpr int kAhead = 4;
+
+template <int DT, int HD, bool CACHE>
+__global__ void __launch_bounds__(kVecThreads) qk_norm_rope_vec_kernel(RopeArgs a, int split) {
+  constexpr int SIZE = DT == QL_F32 ? 4 : 2;
+  constexpr int E = 16 / SIZE > HD / 32 ? 16 / SIZE : HD / 32;
+  constexpr int LPH = HD / E, HPW = 32 / LPH, NV = E * SIZE / 16;
+  const int lane = threadIdx.x & 31, l = lane % LPH, sub = lane / LPH;
+  const long warp = (long)blockIdx.x * (kVecThreads / 32) + (threadIdx.x >> 5);
+  const long t = warp / split;
+  if (t >= a.T) return;
+  const int iq = (a.NH + HPW - 1) / HPW, ik = (a.NKV + HPW - 1) / HPW, steps = iq + (CACHE ? 2 : 1) * ik;
+  const int pos = a.positions[t];
+  const bool in = pos >= 0 && pos < a.lmax;
+  long slot = -1;
+  if (CACHE) slot = a.slots[t];
+  const bool keep = !CACHE || (slot >= 0 && slot < a.num_slots && in);
+  const int hl = a.half / E;                           // lanes of a rotated half
+  const bool first = l < hl, turns = l < 2 * hl;
+  const int partner = lane - l + (first ? l + hl : turns ? l - hl : l);
+  float c[E], sn[E];
+  if (turns && in) {
+    const long row = (long)pos * a.half + (first ? l : l - hl) * E;
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = __ushort_as_half((unsigned short)0);
-    return;
+    for (int i = 0; i < E; i += 4) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(a.cos + row + i));
+      const float4 v = __ldg(reinterpret_cast<const float4*>(a.sin + row + i));
+      c[i] = u.x; c[i + 1] = u.y; c[i + 2] = u.z; c[i + 3] = u.w;
+      sn[i] = v.x; sn[i + 1] = v.y; sn[i + 2] = v.z; sn[i + 3] = v.w;
+    }
   }
-  const int r = (int)(slot & 15), gl = a.group / V;
-  const uint8_t* blk = block_of(a, slot, g, HD) + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
-  const uint8_t* cp = blk + r * (HD / 2) + lane * (V / 2);
-  uint32_t code = V == 2 ? *cp : V == 4 ? *reinterpret_cast<const uint16_t*>(cp) : *reinterpret_cast<const uint32_t*>(cp);
-  const __half2 sm = reinterpret_cast<const __half2*>(blk + code_bytes(HD))[r * (HD / a.group) + lane / gl];
+  uint8_t* blk = nullptr;                              // head 0's block, and the row in it
+  long head_bytes = 0;
+  int r = 0;
+  if (CACHE && keep) {
+    blk = block_of(a, slot, 0, HD);
+    head_bytes = (long)block_bytes(HD, a.group) << (a.page_shift - 4);
+    r = (int)(slot & 15);
+  }
+  const uint8_t* rowp = reinterpret_cast<const uint8_t*>(a.qkv) + t * a.ld * SIZE;
+  // step i: queries, then keys, then values; the head of this lane, or -1
+  const auto head_of = [&](int i) {
+    const int h = i < iq ? i * HPW + sub : (i - iq < ik ? i - iq : i - iq - ik) * HPW + sub;
+    return h < (i < iq ? a.NH : a.NKV) ? h : -1;
+  };
+  for (int i0 = warp % split; i0 < steps; i0 += split * kAhead) {
+    uint4 raw[kAhead][NV];
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    out[i] = __hfma(__int2half_rn((int)((code >> (4 * i)) & 15u)), __low2half(sm), __high2half(sm));
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * split, h = i < steps ? head_of(i) : -1;
+      if (h >= 0 && (i < iq || keep)) {
+        const int col = i < iq ? h : i - iq < ik ? a.NH + h : a.NH + a.NKV + h;
+        const uint4* p = reinterpret_cast<const uint4*>(rowp + ((long)col * HD + l * E) * SIZE);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) raw[u][v] = __ldg(p + v);
+      } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) raw[u][v] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * split;
+      if (i >= steps || !(i < iq || keep)) continue;   // the same for the whole warp
+      const int h = head_of(i);
+      const bool is_q = i < iq, is_v = i >= iq + ik;
+      float x[E];
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const uint32_t w[4] = {raw[u][v].x, raw[u][v].y, raw[u][v].z, raw[u][v].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (DT == QL_F32) {
+            x[4 * v + j] = __int_as_float(w[j]);
+          } else {
+            float2 f;
+            if (DT == QL_F16) f = __half22float2(u32_as_h2(w[j]));
+            else f = make_float2(__int_as_float(w[j] << 16), __int_as_float(w[j] & 0xffff0000u));
+            x[2 * j] = f.x;
+            x[2 * j + 1] = f.y;
+          }
+        }
+      }
+      if (!is_v) {
+        const float* w = is_q ? a.qw : a.kw;
+        if (w) {
+          float s[E];
+#pragma unroll
+          for (int j = 0; j < E; ++j) s[j] = __fmul_rn(x[j], x[j]);
+#pragma unroll
+          for (int n = E; n > 1; n /= 2)
+#pragma unroll
+            for (int j = 0; j < n / 2; ++j) s[j] = __fadd_rn(s[2 * j], s[2 * j + 1]);
+          float ss = s[0];
+#pragma unroll
+          for (int o = 1; o < LPH; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+          const float inv = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
+#pragma unroll
+          for (int j = 0; j < E; j += 4) {
+            const float4 g = __ldg(reinterpret_cast<const float4*>(w + l * E + j));
+            x[j] = __fmul_rn(__fmul_rn(x[j], inv), g.x);
+            x[j + 1] = __fmul_rn(__fmul_rn(x[j + 1], inv), g.y);
+            x[j + 2] = __fmul_rn(__fmul_rn(x[j + 2], inv), g.z);
+            x[j + 3] = __fmul_rn(__fmul_rn(x[j + 3], inv), g.w);
+          }
+        }
+        if (hl > 0) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const float y = __shfl_sync(0xffffffffu, x[j], partner);
+            if (turns && in)
+              x[j] = first ? __fsub_rn(__fmul_rn(x[j], c[j]), __fmul_rn(y, sn[j]))
+                           : __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(y, sn[j]));
+          }
+        }
+        if (!in)
+#pragma unroll
+          for (int j = 0; j < E; ++j) x[j] = pos < 0 ? 0.f : __int_as_float(0x7fc00000);
+      }
+      if (is_q || !CACHE) {
+        if (h < 0) continue;
+        void* out = is_q ? a.q_out : a.k_out;
+        const long at = (t * (is_q ? a.NH : a.NKV) + h) * HD + l * E;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          uint4 o;
+          if (DT == QL_F32) {
+            o = make_uint4(__float_as_uint(x[4 * v]), __float_as_uint(x[4 * v + 1]), __float_as_uint(x[4 * v + 2]),
+                           __float_as_uint(x[4 * v + 3]));
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (DT == QL_F16) {
+                w[j] = h2_as_u32(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
+              } else {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t*>(&b);
+              }
+            }
+            o = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + at * SIZE)[v] = o;
+        }
+        continue;
+      }
+      // 4 bits: minimum and range over the group's lanes; an element that no half holds makes the
+      // maximum infinite
+      const int gl = a.group / E;
+      float lo = x[0], hi = x[0];
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        lo = fminf(lo, x[j]);
+        hi = fmaxf(hi, fabsf(x[j]) <= 65504.f ? x[j] : INFINITY);
+      }
+      for (int o = 1; o < gl; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      const bool ok = hi <= 65504.f;
+      __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)), m = __float2half_rn(lo);
+      if (!ok) s = m = __ushort_as_half((unsigned short)0x7fff);
+      const float sf = __half2float(s), mf = __half2float(m);
+      uint32_t code = 0;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float n = !ok || sf == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], mf), sf)), 0.f), 15.f);
+        code |= (uint32_t)n << (4 * j);
+      }
+      if (h < 0) continue;
+      uint8_t* to = blk + h * head_bytes + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
+      uint8_t* cp = to + r * (HD / 2) + l * (E / 2);
+      if (E == 4) *reinterpret_cast<uint16_t*>(cp) = (uint16_t)code;
+      else *reinterpret_cast<uint32_t*>(cp) = code;
+      if (l % gl == 0)
+        reinterpret_cast<__half2*>(to + code_bytes(HD))[r * (HD / a.group) + l / gl] = __halves2half2(s, m);
+    }
+  }
+}
+
+// The values that slots stand for: a thread decodes one word of 8 codes into 16 bytes.
+template <int HD>
+__global__ void __launch_bounds__(kVecThreads) kv4_read_kernel(RopeArgs a, __half* k_out, __half* v_out) {
+  constexpr int W = HD / 8;
+  const long i = (long)blockIdx.x * kVecThreads + threadIdx.x;
+  const int w = (int)(i % W);
+  const long rest = i / W, t = rest / (2 * a.NKV);
+  if (t >= a.T) return;
+  const int h = (int)(rest - t * 2 * a.NKV);
+  const bool is_v = h >= a.NKV;
+  const int g = is_v ? h - a.NKV : h;
+  const long slot = a.slots[t];
+  uint4 o = make_uint4(0u, 0u, 0u, 0u);
+  if (slot >= 0 && slot < a.num_slots) {
+    const int r = (int)(slot & 15);
+    const uint8_t* blk = block_of(a, slot, g, HD) + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
+    const uint32_t code = *reinterpret_cast<const uint32_t*>(blk + r * (HD / 2) + 4 * w);
+    const __half2 sm = reinterpret_cast<const __half2*>(blk + code_bytes(HD))[r * (HD / a.group) + 8 * w / a.group];
+    __half2 n[4];                                       // (element j, element j + 4)
+    codes_h2(code, n);
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = h2_as_u32(__hfma2(n[j], __low2half2(sm), __high2half2(sm)));
+    o = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                   __byte_perm(v[2], v[3], 0x7632));
+  }
+  reinterpret_cast<uint4*>((is_v ? v_out : k_out) + (t * a.NKV + g) * HD)[w] = o;
 }
 
 bool cache_args(const char* who, const void* cache, int num_pages, int NKV, int HD, int page, int group) {
@@ -178,14 +365,30 @@ bool cache_args(const char* who, const void* cache, int num_pages, int NKV, int 
   return true;
 }
 
-template <int DT>
-cudaError_t launch_rope(const RopeArgs& a, int HD, cudaStream_t st) {
+template <int DT, int HD>
+cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st) {
+  constexpr int SIZE = DT == QL_F32 ? 4 : 2, E = 16 / SIZE > HD / 32 ? 16 / SIZE : HD / 32, HPW = 32 * E / HD;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.qkv) | reinterpret_cast<uintptr_t>(a.q_out) |
+                       reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.cos) |
+                       reinterpret_cast<uintptr_t>(a.sin) | reinterpret_cast<uintptr_t>(a.qw) |
+                       reinterpret_cast<uintptr_t>(a.kw) | (uintptr_t)(a.ld * SIZE);
+  if (at % 16 == 0 && a.half % E == 0) {
+    const int steps = (a.NH + HPW - 1) / HPW + (a.cache ? 2 : 1) * ((a.NKV + HPW - 1) / HPW);
+    // at least 16 warps an SM, as far as there are steps for them
+    const int split = (int)max(1L, min((long)steps, 148L * 16 / a.T));
+    const long blocks = ((long)a.T * split + kVecThreads / 32 - 1) / (kVecThreads / 32);
+    if (a.cache) qk_norm_rope_vec_kernel<DT, HD, true><<<(unsigned)blocks, kVecThreads, 0, st>>>(a, split);
+    else qk_norm_rope_vec_kernel<DT, HD, false><<<(unsigned)blocks, kVecThreads, 0, st>>>(a, split);
+    return cudaGetLastError();
+  }
   const long items = (long)a.T * (a.NH + (a.cache ? 2 * a.NKV : a.NKV));
-  const unsigned blocks = (unsigned)((items + kThreads / 32 - 1) / (kThreads / 32));
-  if (HD == 64) qk_norm_rope_kernel<DT, 64><<<blocks, kThreads, 0, st>>>(a);
-  else if (HD == 128) qk_norm_rope_kernel<DT, 128><<<blocks, kThreads, 0, st>>>(a);
-  else qk_norm_rope_kernel<DT, 256><<<blocks, kThreads, 0, st>>>(a);
+  qk_norm_rope_kernel<DT, HD><<<(unsigned)((items + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(a);
   return cudaGetLastError();
+}
+
+template <int DT>
+cudaError_t launch_rope_hd(const RopeArgs& a, int HD, cudaStream_t st) {
+  return HD == 64 ? launch_rope<DT, 64>(a, st) : HD == 128 ? launch_rope<DT, 128>(a, st) : launch_rope<DT, 256>(a, st);
 }
 
 }  // namespace
@@ -233,16 +436,17 @@ extern "C" int ql_qk_norm_rope(const void* qkv, int dtype, long ld, int T, int N
   a.group = group;
   a.slots = slots;
   const cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = dtype == QL_F32 ? launch_rope<QL_F32>(a, HD, st)
-                        : dtype == QL_F16 ? launch_rope<QL_F16>(a, HD, st) : launch_rope<QL_BF16>(a, HD, st);
+  const cudaError_t e = dtype == QL_F32 ? launch_rope_hd<QL_F32>(a, HD, st)
+                        : dtype == QL_F16 ? launch_rope_hd<QL_F16>(a, HD, st) : launch_rope_hd<QL_BF16>(a, HD, st);
   return cuda_status(e, "ql_qk_norm_rope launch");
 }
 
 extern "C" int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, int page, int group, const int64_t* slots,
                            int T, void* k_out, void* v_out, void* stream) {
   if (T == 0) return QL_OK;
-  if (!cache || !slots || !k_out || !v_out || T < 0) {
-    set_error("ql_kv4_read: bad arguments (T=%d)", T);
+  if (!cache || !slots || !k_out || !v_out || T < 0 ||
+      ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15)) {
+    set_error("ql_kv4_read: bad arguments (T=%d; outputs 16-byte aligned)", T);
     return QL_ERR_ARG;
   }
   if (!cache_args("ql_kv4_read", cache, num_pages, NKV, HD, page, group)) return QL_ERR_ARG;
@@ -254,13 +458,13 @@ extern "C" int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, in
   a.page_shift = __builtin_ctz((unsigned)page);
   a.group = group;
   a.slots = slots;
-  const long items = (long)T * 2 * NKV;
-  const unsigned blocks = (unsigned)((items + kThreads / 32 - 1) / (kThreads / 32));
+  const long words = (long)T * 2 * NKV * (HD / 8);
+  const unsigned blocks = (unsigned)((words + kVecThreads - 1) / kVecThreads);
   const cudaStream_t st = (cudaStream_t)stream;
   __half* k = reinterpret_cast<__half*>(k_out);
   __half* v = reinterpret_cast<__half*>(v_out);
-  if (HD == 64) kv4_read_kernel<64><<<blocks, kThreads, 0, st>>>(a, k, v);
-  else if (HD == 128) kv4_read_kernel<128><<<blocks, kThreads, 0, st>>>(a, k, v);
-  else kv4_read_kernel<256><<<blocks, kThreads, 0, st>>>(a, k, v);
+  if (HD == 64) kv4_read_kernel<64><<<blocks, kVecThreads, 0, st>>>(a, k, v);
+  else if (HD == 128) kv4_read_kernel<128><<<blocks, kVecThreads, 0, st>>>(a, k, v);
+  else kv4_read_kernel<256><<<blocks, kVecThreads, 0, st>>>(a, k, v);
   return cuda_status(cudaGetLastError(), "ql_kv4_read launch");
 }
