@@ -142,96 +142,166 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
     reinterpret_cast<__half2*>(blk + code_bytes(HD))[r * (HD / a.group) + lane / gl] = __halves2half2(s, m);
 }
 
+// rint(d / s) for 0 <= d / s < 2^22 and s a half, as IEEE division rounds it. The product with 1 / s is off by a
+// rounding or two, which matters next to k + 1/2 only, and there the comparison is exact: (k + 1/2) s and
+// d - n s are fp32 numbers, and no d other than (k + 1/2) s itself has a quotient that rounds to k + 1/2 (a
+// neighbour of d is further off, relatively, than half a step of the quotient).
+__device__ __forceinline__ float round_quotient(float d, float s, float inv) {
+  constexpr float kMagic = 12582912.f;             // 1.5 * 2^23: the sum rounds to an integer, ties to even
+  float n = __fsub_rn(__fadd_rn(__fmul_rn(d, inv), kMagic), kMagic);
+  const float rest = fmaf(-n, s, d), half = 0.5f * s;
+  if (fabsf(rest) >= half) {
+    const bool odd = __float_as_int(__fadd_rn(n, kMagic)) & 1;
+    if (fabsf(rest) > half || odd) n += rest > 0.f ? 1.f : -1.f;
+  }
+  return n;
+}
+
 // Rows of 16-byte aligned heads whose rotated halves are whole 16-byte pieces: a lane holds E consecutive
-// elements (16 bytes; 8 fp32 elements at HD = 256), so 16 bytes a lane are read and written, a warp takes 32 E / HD
-// heads at a time, and one token's cos, sin and slot serve all of its heads. `split` warps share a token, so that
-// few tokens still fill the GPU. kAhead loads are under way at once.
+// elements (16 bytes; 8 fp32 elements at HD = 256), so 16 bytes a lane are read and written, a warp takes
+// 32 E / HD heads at a time, and one token's cos, sin and slot serve all of its heads. `split` warps share a
+// token, so that few tokens still fill the GPU. kAhead loads are under way at once.
 constexpr int kVecThreads = 256;
 constexpr int kAhead = 4;
 
-template <int DT, int HD, bool CACHE>
-__global__ void __launch_bounds__(kVecThreads) qk_norm_rope_vec_kernel(RopeArgs a, int split) {
-  constexpr int SIZE = DT == QL_F32 ? 4 : 2;
-  constexpr int E = 16 / SIZE > HD / 32 ? 16 / SIZE : HD / 32;
-  constexpr int LPH = HD / E, HPW = 32 / LPH, NV = E * SIZE / 16;
-  const int lane = threadIdx.x & 31, l = lane % LPH, sub = lane / LPH;
-  const long warp = (long)blockIdx.x * (kVecThreads / 32) + (threadIdx.x >> 5);
-  const long t = warp / split;
-  if (t >= a.T) return;
-  const int iq = (a.NH + HPW - 1) / HPW, ik = (a.NKV + HPW - 1) / HPW, steps = iq + (CACHE ? 2 : 1) * ik;
-  const int pos = a.positions[t];
-  const bool in = pos >= 0 && pos < a.lmax;
-  long slot = -1;
-  if (CACHE) slot = a.slots[t];
-  const bool keep = !CACHE || (slot >= 0 && slot < a.num_slots && in);
-  const int hl = a.half / E;                           // lanes of a rotated half
-  const bool first = l < hl, turns = l < 2 * hl;
-  const int partner = lane - l + (first ? l + hl : turns ? l - hl : l);
-  float c[E], sn[E];
-  if (turns && in) {
-    const long row = (long)pos * a.half + (first ? l : l - hl) * E;
+template <int DT, int HD>
+struct Lanes {
+  static constexpr int SIZE = DT == QL_F32 ? 4 : 2;
+  static constexpr int E = 16 / SIZE > HD / 32 ? 16 / SIZE : HD / 32;
+  static constexpr int LPH = HD / E, HPW = 32 / LPH, NV = E * SIZE / 16;
+};
+
+template <int DT, int HD>
+struct Token {
+  long t;
+  int pos;
+  bool in;                       // a position of the tables
+  const uint8_t* row;
+  float c[Lanes<DT, HD>::E], s[Lanes<DT, HD>::E];   // of this lane's elements; s with the sign of its half
+  int partner;                   // the lane with the other half's elements
+  bool turns;                    // this lane's elements are rotated
+  uint8_t* blk;                  // head 0's block in the cache
+  long head_bytes;
+  int r;                         // row in the block
+};
+
+template <int DT, int HD>
+__device__ __forceinline__ void unpack(const uint4 (&raw)[Lanes<DT, HD>::NV], float (&x)[Lanes<DT, HD>::E]) {
 #pragma unroll
-    for (int i = 0; i < E; i += 4) {
-      const float4 u = __ldg(reinterpret_cast<const float4*>(a.cos + row + i));
-      const float4 v = __ldg(reinterpret_cast<const float4*>(a.sin + row + i));
-      c[i] = u.x; c[i + 1] = u.y; c[i + 2] = u.z; c[i + 3] = u.w;
-      sn[i] = v.x; sn[i + 1] = v.y; sn[i + 2] = v.z; sn[i + 3] = v.w;
-    }
-  }
-  uint8_t* blk = nullptr;                              // head 0's block, and the row in it
-  long head_bytes = 0;
-  int r = 0;
-  if (CACHE && keep) {
-    blk = block_of(a, slot, 0, HD);
-    head_bytes = (long)block_bytes(HD, a.group) << (a.page_shift - 4);
-    r = (int)(slot & 15);
-  }
-  const uint8_t* rowp = reinterpret_cast<const uint8_t*>(a.qkv) + t * a.ld * SIZE;
-  // step i: queries, then keys, then values; the head of this lane, or -1
-  const auto head_of = [&](int i) {
-    const int h = i < iq ? i * HPW + sub : (i - iq < ik ? i - iq : i - iq - ik) * HPW + sub;
-    return h < (i < iq ? a.NH : a.NKV) ? h : -1;
-  };
-  for (int i0 = warp % split; i0 < steps; i0 += split * kAhead) {
-    uint4 raw[kAhead][NV];
+  for (int v = 0; v < Lanes<DT, HD>::NV; ++v) {
+    const uint32_t w[4] = {raw[v].x, raw[v].y, raw[v].z, raw[v].w};
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u * split, h = i < steps ? head_of(i) : -1;
-      if (h >= 0 && (i < iq || keep)) {
-        const int col = i < iq ? h : i - iq < ik ? a.NH + h : a.NH + a.NKV + h;
-        const uint4* p = reinterpret_cast<const uint4*>(rowp + ((long)col * HD + l * E) * SIZE);
-#pragma unroll
-        for (int v = 0; v < NV; ++v) raw[u][v] = __ldg(p + v);
+    for (int j = 0; j < 4; ++j) {
+      if (DT == QL_F32) {
+        x[4 * v + j] = __int_as_float(w[j]);
       } else {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) raw[u][v] = make_uint4(0u, 0u, 0u, 0u);
+        const float2 f = DT == QL_F16 ? __half22float2(u32_as_h2(w[j]))
+                                      : make_float2(__int_as_float(w[j] << 16), __int_as_float(w[j] & 0xffff0000u));
+        x[2 * j] = f.x;
+        x[2 * j + 1] = f.y;
       }
+    }
+  }
+}
+
+template <int DT, int HD>
+__device__ __forceinline__ void store_head(void* out, long at, const float (&x)[Lanes<DT, HD>::E]) {
+  uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + at * Lanes<DT, HD>::SIZE);
+#pragma unroll
+  for (int v = 0; v < Lanes<DT, HD>::NV; ++v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (DT == QL_F32) {
+        w[j] = __float_as_uint(x[4 * v + j]);
+      } else if (DT == QL_F16) {
+        w[j] = h2_as_u32(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
+      } else {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    }
+    p[v] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// A head's elements in 4 bits: minimum and range over the group's lanes; an element that no half holds
+// makes the maximum infinite.
+template <int DT, int HD>
+__device__ __forceinline__ void store_codes(const RopeArgs& a, const Token<DT, HD>& k, int h, bool is_v, int l,
+                                            const float (&x)[Lanes<DT, HD>::E]) {
+  constexpr int E = Lanes<DT, HD>::E;
+  const int gl = a.group / E;
+  float lo = x[0], hi = x[0], most = fabsf(x[0]);
+  bool ok = most <= 65504.f;
+#pragma unroll
+  for (int j = 1; j < E; ++j) {
+    lo = fminf(lo, x[j]);
+    hi = fmaxf(hi, x[j]);
+    if (DT != QL_F16) ok = ok && fabsf(x[j]) <= 65504.f;
+    else ok = ok && fabsf(x[j]) < INFINITY;
+  }
+  if (!ok) hi = INFINITY;
+  for (int o = 1; o < gl; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  ok = hi <= 65504.f;
+  __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)), m = __float2half_rn(lo);
+  if (!ok) s = m = __ushort_as_half((unsigned short)0x7fff);
+  const float sf = __half2float(s), mf = __half2float(m);
+  const bool flat = !(sf > 0.f);                     // constant, or not finite: codes 0
+  const float inv = flat ? 0.f : __frcp_rn(sf), step = flat ? 1.f : sf;
+  uint32_t code = 0;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    // below zero by the minimum's rounding, above 15 by the scale's
+    const float d = flat ? 0.f : fminf(fmaxf(__fsub_rn(x[j], mf), 0.f), 15.f * step);
+    code |= (uint32_t)__float2int_rn(round_quotient(d, step, inv)) << (4 * j);
+  }
+  if (h < 0) return;
+  uint8_t* to = k.blk + h * k.head_bytes + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
+  uint8_t* cp = to + k.r * (HD / 2) + l * (E / 2);
+  if (E == 4) *reinterpret_cast<uint16_t*>(cp) = (uint16_t)code;
+  else *reinterpret_cast<uint32_t*>(cp) = code;
+  if ((l & (gl - 1)) == 0)
+    reinterpret_cast<__half2*>(to + code_bytes(HD))[k.r * (HD / a.group) + l / gl] = __halves2half2(s, m);
+}
+
+enum { kQuery, kKey, kValue };
+
+// Steps i0 .. i1 - 1 of one kind of heads, HPW heads a step.
+template <int DT, int HD, bool CACHE, bool FULL, int KIND>
+__device__ __forceinline__ void heads(const RopeArgs& a, const Token<DT, HD>& k, int i0, int i1) {
+  using L = Lanes<DT, HD>;
+  constexpr int E = L::E;
+  const int lane = threadIdx.x & 31, l = lane % L::LPH, sub = lane / L::LPH;
+  const int count = KIND == kQuery ? a.NH : a.NKV, first = KIND == kQuery ? 0 : KIND == kKey ? a.NH : a.NH + a.NKV;
+  const float* w = KIND == kQuery ? a.qw : KIND == kKey ? a.kw : nullptr;
+  const uint8_t* from = k.row + ((long)first * HD + l * E) * L::SIZE;
+  float g[E];
+  if (w)
+#pragma unroll
+    for (int j = 0; j < E; j += 4) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(w + l * E + j));
+      g[j] = u.x; g[j + 1] = u.y; g[j + 2] = u.z; g[j + 3] = u.w;
+    }
+  for (; i0 < i1; i0 += kAhead) {
+    uint4 raw[kAhead][L::NV];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int h = min((i0 + u) * L::HPW + sub, count - 1);   // past the last head: it again, not stored
+      const uint4* p = reinterpret_cast<const uint4*>(from + (long)h * (HD * L::SIZE));
+#pragma unroll
+      for (int v = 0; v < L::NV; ++v) raw[u][v] = __ldg(p + v);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u * split;
-      if (i >= steps || !(i < iq || keep)) continue;   // the same for the whole warp
-      const int h = head_of(i);
-      const bool is_q = i < iq, is_v = i >= iq + ik;
+      if (i0 + u >= i1) break;
+      const int h = (i0 + u) * L::HPW + sub < count ? (i0 + u) * L::HPW + sub : -1;
       float x[E];
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const uint32_t w[4] = {raw[u][v].x, raw[u][v].y, raw[u][v].z, raw[u][v].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (DT == QL_F32) {
-            x[4 * v + j] = __int_as_float(w[j]);
-          } else {
-            float2 f;
-            if (DT == QL_F16) f = __half22float2(u32_as_h2(w[j]));
-            else f = make_float2(__int_as_float(w[j] << 16), __int_as_float(w[j] & 0xffff0000u));
-            x[2 * j] = f.x;
-            x[2 * j + 1] = f.y;
-          }
-        }
-      }
-      if (!is_v) {
-        const float* w = is_q ? a.qw : a.kw;
+      unpack<DT, HD>(raw[u], x);
+      if (KIND != kValue) {
         if (w) {
           float s[E];
 #pragma unroll
@@ -242,118 +312,107 @@ __global__ void __launch_bounds__(kVecThreads) qk_norm_rope_vec_kernel(RopeArgs 
             for (int j = 0; j < n / 2; ++j) s[j] = __fadd_rn(s[2 * j], s[2 * j + 1]);
           float ss = s[0];
 #pragma unroll
-          for (int o = 1; o < LPH; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
-          const float inv = __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
+          for (int o = 1; o < L::LPH; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+          const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
 #pragma unroll
-          for (int j = 0; j < E; j += 4) {
-            const float4 g = __ldg(reinterpret_cast<const float4*>(w + l * E + j));
-            x[j] = __fmul_rn(__fmul_rn(x[j], inv), g.x);
-            x[j + 1] = __fmul_rn(__fmul_rn(x[j + 1], inv), g.y);
-            x[j + 2] = __fmul_rn(__fmul_rn(x[j + 2], inv), g.z);
-            x[j + 3] = __fmul_rn(__fmul_rn(x[j + 3], inv), g.w);
-          }
+          for (int j = 0; j < E; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], inv), g[j]);
         }
-        if (hl > 0) {
 #pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const float y = __shfl_sync(0xffffffffu, x[j], partner);
-            if (turns && in)
-              x[j] = first ? __fsub_rn(__fmul_rn(x[j], c[j]), __fmul_rn(y, sn[j]))
-                           : __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(y, sn[j]));
-          }
+        for (int j = 0; j < E; ++j) {
+          // x c - y s is x c + y (-s) to the bit
+          const float y = __shfl_sync(0xffffffffu, x[j], k.partner);
+          const float z = __fadd_rn(__fmul_rn(x[j], k.c[j]), __fmul_rn(y, k.s[j]));
+          x[j] = FULL || k.turns ? z : x[j];
         }
-        if (!in)
+        if (!k.in)
 #pragma unroll
-          for (int j = 0; j < E; ++j) x[j] = pos < 0 ? 0.f : __int_as_float(0x7fc00000);
+          for (int j = 0; j < E; ++j) x[j] = k.pos < 0 ? 0.f : __int_as_float(0x7fc00000);
       }
-      if (is_q || !CACHE) {
-        if (h < 0) continue;
-        void* out = is_q ? a.q_out : a.k_out;
-        const long at = (t * (is_q ? a.NH : a.NKV) + h) * HD + l * E;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          uint4 o;
-          if (DT == QL_F32) {
-            o = make_uint4(__float_as_uint(x[4 * v]), __float_as_uint(x[4 * v + 1]), __float_as_uint(x[4 * v + 2]),
-                           __float_as_uint(x[4 * v + 3]));
-          } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (DT == QL_F16) {
-                w[j] = h2_as_u32(__floats2half2_rn(x[2 * j], x[2 * j + 1]));
-              } else {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-                w[j] = *reinterpret_cast<const uint32_t*>(&b);
-              }
-            }
-            o = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-          reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + at * SIZE)[v] = o;
-        }
-        continue;
+      if (KIND == kQuery || !CACHE) {
+        if (h >= 0) store_head<DT, HD>(KIND == kQuery ? a.q_out : a.k_out, (k.t * count + h) * HD + l * E, x);
+      } else {
+        store_codes<DT, HD>(a, k, h, KIND == kValue, l, x);
       }
-      // 4 bits: minimum and range over the group's lanes; an element that no half holds makes the
-      // maximum infinite
-      const int gl = a.group / E;
-      float lo = x[0], hi = x[0];
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        lo = fminf(lo, x[j]);
-        hi = fmaxf(hi, fabsf(x[j]) <= 65504.f ? x[j] : INFINITY);
-      }
-      for (int o = 1; o < gl; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      }
-      const bool ok = hi <= 65504.f;
-      __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)), m = __float2half_rn(lo);
-      if (!ok) s = m = __ushort_as_half((unsigned short)0x7fff);
-      const float sf = __half2float(s), mf = __half2float(m);
-      uint32_t code = 0;
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float n = !ok || sf == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], mf), sf)), 0.f), 15.f);
-        code |= (uint32_t)n << (4 * j);
-      }
-      if (h < 0) continue;
-      uint8_t* to = blk + h * head_bytes + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
-      uint8_t* cp = to + r * (HD / 2) + l * (E / 2);
-      if (E == 4) *reinterpret_cast<uint16_t*>(cp) = (uint16_t)code;
-      else *reinterpret_cast<uint32_t*>(cp) = code;
-      if (l % gl == 0)
-        reinterpret_cast<__half2*>(to + code_bytes(HD))[r * (HD / a.group) + l / gl] = __halves2half2(s, m);
     }
   }
 }
 
-// The values that slots stand for: a thread decodes one word of 8 codes into 16 bytes.
+template <int DT, int HD, bool CACHE, bool FULL>
+__global__ void __launch_bounds__(kVecThreads) qk_norm_rope_vec_kernel(RopeArgs a, int split) {
+  using L = Lanes<DT, HD>;
+  constexpr int E = L::E;
+  const int lane = threadIdx.x & 31, l = lane % L::LPH;
+  const unsigned warp = blockIdx.x * (kVecThreads / 32) + (threadIdx.x >> 5);
+  const unsigned t = warp / (unsigned)split, part = warp - t * (unsigned)split;
+  if (t >= (unsigned)a.T) return;
+  Token<DT, HD> k;
+  k.t = t;
+  k.pos = a.positions[t];
+  k.in = k.pos >= 0 && k.pos < a.lmax;
+  k.row = reinterpret_cast<const uint8_t*>(a.qkv) + t * a.ld * L::SIZE;
+  const int hl = a.half / E;                           // lanes of a rotated half
+  const bool first = l < hl;
+  k.turns = l < 2 * hl;
+  k.partner = lane - l + (first ? l + hl : k.turns ? l - hl : l);
+#pragma unroll
+  for (int j = 0; j < E; ++j) k.c[j] = k.s[j] = 0.f;
+  if (k.turns && k.in) {
+    const long row = (long)k.pos * a.half + (first ? l : l - hl) * E;
+    const float sign = first ? -1.f : 1.f;
+#pragma unroll
+    for (int j = 0; j < E; j += 4) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(a.cos + row + j));
+      const float4 v = __ldg(reinterpret_cast<const float4*>(a.sin + row + j));
+      k.c[j] = u.x; k.c[j + 1] = u.y; k.c[j + 2] = u.z; k.c[j + 3] = u.w;
+      k.s[j] = sign * v.x; k.s[j + 1] = sign * v.y; k.s[j + 2] = sign * v.z; k.s[j + 3] = sign * v.w;
+    }
+  }
+  const int iq = (a.NH + L::HPW - 1) / L::HPW, ik = (a.NKV + L::HPW - 1) / L::HPW, steps = iq + (CACHE ? 2 : 1) * ik;
+  const int i0 = (int)(part * steps / split), i1 = (int)((part + 1) * steps / split);
+  if (i0 < iq) heads<DT, HD, CACHE, FULL, kQuery>(a, k, i0, min(i1, iq));
+  if (i1 <= iq) return;
+  if (CACHE) {
+    const long slot = a.slots[t];
+    if (slot < 0 || slot >= a.num_slots || !k.in) return;   // not cached
+    k.blk = block_of(a, slot, 0, HD);
+    k.head_bytes = (long)block_bytes(HD, a.group) << (a.page_shift - 4);
+    k.r = (int)(slot & 15);
+  }
+  if (i0 < iq + ik) heads<DT, HD, CACHE, FULL, kKey>(a, k, max(i0 - iq, 0), min(i1 - iq, ik));
+  if (CACHE && i1 > iq + ik) heads<DT, HD, CACHE, FULL, kValue>(a, k, max(i0 - iq - ik, 0), i1 - iq - ik);
+}
+
+// The values that slots stand for: a warp takes a token, a lane decodes words of 8 codes into 16 bytes.
 template <int HD>
 __global__ void __launch_bounds__(kVecThreads) kv4_read_kernel(RopeArgs a, __half* k_out, __half* v_out) {
   constexpr int W = HD / 8;
-  const long i = (long)blockIdx.x * kVecThreads + threadIdx.x;
-  const int w = (int)(i % W);
-  const long rest = i / W, t = rest / (2 * a.NKV);
+  const long t = (long)blockIdx.x * (kVecThreads / 32) + (threadIdx.x >> 5);
   if (t >= a.T) return;
-  const int h = (int)(rest - t * 2 * a.NKV);
-  const bool is_v = h >= a.NKV;
-  const int g = is_v ? h - a.NKV : h;
   const long slot = a.slots[t];
-  uint4 o = make_uint4(0u, 0u, 0u, 0u);
-  if (slot >= 0 && slot < a.num_slots) {
-    const int r = (int)(slot & 15);
-    const uint8_t* blk = block_of(a, slot, g, HD) + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
-    const uint32_t code = *reinterpret_cast<const uint32_t*>(blk + r * (HD / 2) + 4 * w);
-    const __half2 sm = reinterpret_cast<const __half2*>(blk + code_bytes(HD))[r * (HD / a.group) + 8 * w / a.group];
-    __half2 n[4];                                       // (element j, element j + 4)
-    codes_h2(code, n);
-    uint32_t v[4];
+  const bool in = slot >= 0 && slot < a.num_slots;
+  const int r = (int)(slot & 15);
+  const uint8_t* blk = in ? block_of(a, slot, 0, HD) : nullptr;
+  const long head_bytes = (long)block_bytes(HD, a.group) << (a.page_shift - 4);
+#pragma unroll 2
+  for (int i = threadIdx.x & 31; i < 2 * a.NKV * W; i += 32) {
+    const int h = i / W, w = i % W;
+    const bool is_v = h >= a.NKV;
+    const int g = is_v ? h - a.NKV : h;
+    uint4 o = make_uint4(0u, 0u, 0u, 0u);
+    if (in) {
+      const uint8_t* p = blk + g * head_bytes + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
+      const uint32_t code = *reinterpret_cast<const uint32_t*>(p + r * (HD / 2) + 4 * w);
+      const __half2 sm = reinterpret_cast<const __half2*>(p + code_bytes(HD))[r * (HD / a.group) + 8 * w / a.group];
+      __half2 n[4];                                       // (element j, element j + 4)
+      codes_h2(code, n);
+      uint32_t v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = h2_as_u32(__hfma2(n[j], __low2half2(sm), __high2half2(sm)));
-    o = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
-                   __byte_perm(v[2], v[3], 0x7632));
+      for (int j = 0; j < 4; ++j) v[j] = h2_as_u32(__hfma2(n[j], __low2half2(sm), __high2half2(sm)));
+      o = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                     __byte_perm(v[2], v[3], 0x7632));
+    }
+    reinterpret_cast<uint4*>((is_v ? v_out : k_out) + (t * a.NKV + g) * HD)[w] = o;
   }
-  reinterpret_cast<uint4*>((is_v ? v_out : k_out) + (t * a.NKV + g) * HD)[w] = o;
 }
 
 bool cache_args(const char* who, const void* cache, int num_pages, int NKV, int HD, int page, int group) {
@@ -367,7 +426,7 @@ bool cache_args(const char* who, const void* cache, int num_pages, int NKV, int 
 
 template <int DT, int HD>
 cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st) {
-  constexpr int SIZE = DT == QL_F32 ? 4 : 2, E = 16 / SIZE > HD / 32 ? 16 / SIZE : HD / 32, HPW = 32 * E / HD;
+  constexpr int SIZE = Lanes<DT, HD>::SIZE, E = Lanes<DT, HD>::E, HPW = Lanes<DT, HD>::HPW;
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.qkv) | reinterpret_cast<uintptr_t>(a.q_out) |
                        reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.cos) |
                        reinterpret_cast<uintptr_t>(a.sin) | reinterpret_cast<uintptr_t>(a.qw) |
@@ -377,8 +436,9 @@ cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st) {
     // at least 16 warps an SM, as far as there are steps for them
     const int split = (int)max(1L, min((long)steps, 148L * 16 / a.T));
     const long blocks = ((long)a.T * split + kVecThreads / 32 - 1) / (kVecThreads / 32);
-    if (a.cache) qk_norm_rope_vec_kernel<DT, HD, true><<<(unsigned)blocks, kVecThreads, 0, st>>>(a, split);
-    else qk_norm_rope_vec_kernel<DT, HD, false><<<(unsigned)blocks, kVecThreads, 0, st>>>(a, split);
+    auto kern = a.half * 2 == HD ? (a.cache ? qk_norm_rope_vec_kernel<DT, HD, true, true> : qk_norm_rope_vec_kernel<DT, HD, false, true>)
+                                 : (a.cache ? qk_norm_rope_vec_kernel<DT, HD, true, false> : qk_norm_rope_vec_kernel<DT, HD, false, false>);
+    kern<<<(unsigned)blocks, kVecThreads, 0, st>>>(a, split);
     return cudaGetLastError();
   }
   const long items = (long)a.T * (a.NH + (a.cache ? 2 * a.NKV : a.NKV));
@@ -458,8 +518,7 @@ extern "C" int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, in
   a.page_shift = __builtin_ctz((unsigned)page);
   a.group = group;
   a.slots = slots;
-  const long words = (long)T * 2 * NKV * (HD / 8);
-  const unsigned blocks = (unsigned)((words + kVecThreads - 1) / kVecThreads);
+  const unsigned blocks = (unsigned)(((long)T + kVecThreads / 32 - 1) / (kVecThreads / 32));
   const cudaStream_t st = (cudaStream_t)stream;
   __half* k = reinterpret_cast<__half*>(k_out);
   __half* v = reinterpret_cast<__half*>(v_out);
