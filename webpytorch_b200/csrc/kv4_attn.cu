@@ -23,8 +23,7 @@
 // 64), keeps the running maximum and sum of the tile, writes a tile that it holds whole, and leaves a part of
 // a tile to be joined: first with the parts of the CTA's other warps, then, for at most two tiles a
 // CTA, with those of other CTAs by whichever of them finishes last, always in the same order.
-#include "kv4_common.cuh"
-#include "sm100_ptx.cuh"
+#include "kv4_attn.cuh"
 
 namespace ql {
 
@@ -36,25 +35,7 @@ namespace {
 using namespace kv4;
 
 constexpr int kMaxCtas = 512;   // counters in the workspace
-
-struct AttnArgs {
-  const void* q;
-  long ldq;
-  int T, NH, NKV;
-  const uint8_t* cache;
-  int num_pages, page_shift;
-  const int32_t* table;
-  long table_stride;
-  int width;
-  const int32_t* seq_lens;
-  const int32_t* cu_q;
-  int B;
-  float scale;
-  int window;
-  void* out;
-  unsigned int* counters;   // [kMaxCtas], zero between launches
-  float* parts;             // [ctas][2 + warps] partial results
-};
+constexpr int kPromptRows = 64;
 
 // Warps of a CTA by the registers that a head's state takes, and ring stages by what they leave.
 template <int HD>
@@ -86,8 +67,6 @@ struct Smem {
   static constexpr int kBytes = kBar + Shape<HD>::kWarps * Shape<HD>::kStages * 8;
 };
 
-__device__ __forceinline__ int cu(const AttnArgs& a, int b) { return a.cu_q ? min(max(a.cu_q[b], 0), a.T) : min(b, a.T); }
-
 struct Request {
   int q0, ql, seq;       // first query row, queries, length
   int tiles, blo, nblk;  // row tiles; first block that any query sees, and blocks from there
@@ -100,7 +79,8 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, int b) {
   r.ql = max(cu(a, b + 1) - r.q0, 0);
   r.seq = max(a.seq_lens[b], 0);
   const int end = min(r.seq, a.width << a.page_shift);
-  r.tiles = (r.ql * (a.NH / a.NKV) + ROWS - 1) / ROWS;
+  const int rows = r.ql * (a.NH / a.NKV);
+  r.tiles = a.prompt_rows && rows >= a.prompt_rows ? 0 : (rows + ROWS - 1) / ROWS;
   r.blo = a.window ? max(r.seq - r.ql - a.window + 1, 0) / kBlock : 0;
   r.nblk = max((end + kBlock - 1) / kBlock - r.blo, 1);
   return r;
@@ -491,29 +471,6 @@ struct Piece {
   int b, kvh, r0, nrows, lo_all, hi_all;
   int head, whole;              // its first tile began in an earlier warp; and goes on past this one
 };
-
-constexpr uint32_t kNoBlock = 0xffffffffu;
-
-// Block i of n from blk0 of request b, as its index in the cache; kNoBlock past the end or for a page
-// that is not one of the cache's.
-__device__ __forceinline__ uint32_t source(const AttnArgs& a, int b, int kvh, int blk0, int i, int n) {
-  const int shift = a.page_shift - 4;
-  if (i >= n) return kNoBlock;
-  const int page = a.table[b * a.table_stride + ((blk0 + i) >> shift)];
-  if (page < 0 || page >= a.num_pages) return kNoBlock;
-  return (((uint32_t)page * a.NKV + kvh) << shift) + ((blk0 + i) & ((1 << shift) - 1));
-}
-
-// A lane's block into a stage of the ring.
-template <int BB>
-__device__ __forceinline__ void issue(const AttnArgs& a, uint32_t src, int stage, uint32_t ring, uint32_t bar) {
-  if (src != kNoBlock) {
-    ptx::mbar_arrive_expect_tx(bar + 8 * stage, BB);
-    ptx::bulk_load(ring + stage * BB, a.cache + (size_t)src * BB, BB, bar + 8 * stage);
-  } else {
-    ptx::mbar_arrive(bar + 8 * stage);
-  }
-}
 
 struct Cross {          // a tile that this CTA shares with others
   int valid, q0, kvh, r0, nrows, first, last, finish;
@@ -925,7 +882,7 @@ int take_kv4_status() {
   int v = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&v, g_kv4_status, sizeof(int)) != cudaSuccess) return 0;
   if (v) cudaMemcpyToSymbol(g_kv4_status, &zero, sizeof(int));
-  return v;
+  return v | take_kv4_prompt_status();
 }
 
 }  // namespace ql
@@ -987,10 +944,19 @@ extern "C" int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int N
   a.B = B;
   a.scale = scale;
   a.window = window;
+  // at least half of a prompt tile's rows; the host knows only that no request has more than T - B + 1 tokens
+  // where each has one
+  a.prompt_rows = dtype != QL_F32 && HD <= 128 && (long)T * (NH / NKV) >= kPromptRows ? kPromptRows : 0;
   a.out = out;
   a.counters = reinterpret_cast<unsigned int*>(workspace);
   a.parts = reinterpret_cast<float*>(a.counters + kMaxCtas);
   const cudaStream_t st = (cudaStream_t)stream;
+  if (a.prompt_rows && cu_q) {
+    const int rc = kv4_prompt_attention(a, dtype, HD, group, st);
+    if (rc) return rc;
+  } else {
+    a.prompt_rows = 0;
+  }
   return dtype == QL_F32   ? launch_sizes<QL_F32>(a, HD, group, ctas, st)
          : dtype == QL_F16 ? launch_sizes<QL_F16>(a, HD, group, ctas, st)
                            : launch_sizes<QL_BF16>(a, HD, group, ctas, st);

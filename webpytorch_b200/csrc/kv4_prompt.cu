@@ -1,0 +1,461 @@
+// Attention of prompt chunks over the paged 4-bit cache on the 5th-generation tensor cores: fp16 or
+// bf16 queries of a request that fill kPromptRows rows (query tokens x heads of a key/value head) or
+// more, HD 64 or 128. The other requests of a call are the streaming kernel's.
+//
+// A CTA takes two tiles of 128 rows of one request and key/value head and walks the positions they see
+// in steps of 128:
+//   S = Q K^T  (tcgen05, 128 x 128, Q and K in shared memory)      softmax  P = 2^(coef S - m)
+//   O = O + P V  (P from tensor memory, where it takes the place of S; V in shared memory)
+// The tiles alternate, so the tensor cores work on one while the other is in its softmax. Warps 0 - 3 and
+// 4 - 7 are the tiles' softmax, a thread a row; warps 8 - 11 decode keys and values, once for both tiles;
+// warp 12 issues the MMAs. The running maximum moves only when it grows by more than 2^kLazy, and
+// then the row's O in tensor memory is scaled.
+// What the codes stand for is an fp16 number, so K and V are exact; probabilities are rounded to fp16's
+// 11 bits (outputs have 11 or 8), and sums are fp32.
+// Shared memory holds K and V as [position][element] with the 128-byte swizzle: K-major rows for S, and
+// the same layout read as MN-major for P V. The order of a position's elements is free (the contraction of
+// S; the columns of O), so it is the one in which a lane's 16-byte load of 32 codes gives four 16-byte
+// stores without bank conflicts.
+#include "kv4_common.cuh"
+#include "kv4_attn.cuh"
+#include "sm100_ptx.cuh"
+
+namespace ql {
+
+__device__ int g_kv4_prompt_status = 0;
+
+namespace {
+
+using namespace kv4;
+
+constexpr int kTileRows = 128, kTiles = 2, kStep = 128;
+constexpr int kSoftWarps = 8, kDecodeWarps = 4, kWarps = kSoftWarps + kDecodeWarps + 1, kThreads = kWarps * 32;
+constexpr int kRing = 3;                        // blocks of a decoding warp in flight
+
+template <int HD, int G>
+struct Smem {
+  static constexpr int kPanel = 128 * 128;      // 128 rows of 128 bytes
+  static constexpr int kTile = kPanel * HD / 64;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + kTiles * kTile;
+  static constexpr int kV = kK + 2 * kTile;
+  static constexpr int kRaw = kV + 2 * kTile;
+  static constexpr int kBar = kRaw + kDecodeWarps * kRing * block_bytes(HD, G);
+  // s_full[2], p_full[2], k_full[2], v_full[2], k_free[2], v_free[2], q_full, done, ring[4][3]
+  static constexpr int kBars = 14 + kDecodeWarps * kRing;
+  static constexpr int kMisc = kBar + kBars * 8;
+  static constexpr int kBytes = kMisc + 16 + 1024;   // + alignment slack
+};
+
+// Chunk (16 bytes, one word of 8 codes) of a row: word w of the row is at panel, column.
+template <int HD>
+__device__ __forceinline__ constexpr int panel_of(int w) { return HD == 64 ? 0 : (w & 3) >> 1; }
+template <int HD>
+__device__ __forceinline__ constexpr int column_of(int w) { return HD == 64 ? w : 2 * (w >> 2) + (w & 1); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int DT, int HD, int G>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
+  using L = Smem<HD, G>;
+  constexpr int BB = block_bytes(HD, G), W = HD / 8;
+  constexpr float kLazy = 6.f, kPShift = 9.f;
+  const int grp = a.NH / a.NKV;
+  // tiles of the longest rows first
+  const int kvh = blockIdx.x % a.NKV, x = gridDim.x / a.NKV - 1 - blockIdx.x / a.NKV;
+  constexpr int kRows = kTiles * kTileRows;
+  const auto tile_start = [&](int b) { return (int)((long)cu(a, b) * grp / kRows) + b; };
+  int b = 0;
+  for (int hi = a.B - 1; b < hi;) {               // the last request whose first pair of tiles is at or before x
+    const int mid = (b + hi + 1) >> 1;
+    if (tile_start(mid) <= x) b = mid;
+    else hi = mid - 1;
+  }
+  const int q0 = cu(a, b), ql = max(cu(a, b + 1) - q0, 0), rows = ql * grp, r0 = (x - tile_start(b)) * kRows;
+  if (rows < a.prompt_rows || r0 >= rows) return;
+  const int nrows = min(kRows, rows - r0);
+  const int seq = max(a.seq_lens[b], 0), table_end = a.width << a.page_shift;
+  const int p_first = seq - ql + r0 / grp, p_last = seq - ql + (r0 + nrows - 1) / grp;
+  const int lo_all = a.window ? max(p_first - a.window + 1, 0) : 0, hi_all = min(p_last + 1, table_end);
+  const int blk0 = lo_all / kBlock, nblk = max((hi_all + kBlock - 1) / kBlock - blk0, 0);
+  const int steps = (nblk + kStep / kBlock - 1) / (kStep / kBlock);
+
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = ptx::smem_addr(smem), bar0 = sbase + L::kBar;
+  const auto s_full = [&](int i) { return bar0 + 8u * i; };
+  const auto p_full = [&](int i) { return bar0 + 8u * (2 + i); };
+  const auto k_full = [&](int s) { return bar0 + 8u * (4 + s); };
+  const auto v_full = [&](int s) { return bar0 + 8u * (6 + s); };
+  const auto k_free = [&](int s) { return bar0 + 8u * (8 + s); };
+  const auto v_free = [&](int s) { return bar0 + 8u * (10 + s); };
+  const uint32_t q_full = bar0 + 8u * 12, done = bar0 + 8u * 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+  volatile int* bad_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 8);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(s_full(i), 1);
+      ptx::mbar_init(p_full(i), 4);
+      ptx::mbar_init(k_full(i), kDecodeWarps);
+      ptx::mbar_init(v_full(i), kDecodeWarps);
+      ptx::mbar_init(k_free(i), 1);
+      ptx::mbar_init(v_free(i), 1);
+    }
+    ptx::mbar_init(q_full, kSoftWarps);
+    ptx::mbar_init(done, 1);
+    for (int i = 0; i < kDecodeWarps * kRing; ++i) ptx::mbar_init(bar0 + 8u * (14 + i), 1);
+    *abort_flag = 0;
+    *bad_flag = seq > table_end;                  // a length past the table: nan
+    ptx::fence_mbar_init();
+  }
+  if (warp == kWarps - 1) {
+    ptx::tmem_alloc(ptx::smem_addr(tmem_slot), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // tensor memory of tile i: S (and P over it) at 256 i, O at 256 i + 128
+
+  if (warp < kSoftWarps) {
+    // ---------------- softmax: a thread a row
+    const int tile = warp >> 2, row = (warp & 3) * 32 + lane, i = tile * kTileRows + row;
+    const bool live = i < nrows;
+    const int mine = r0 + min(i, nrows - 1);      // rows past the last repeat it and are not written
+    const int tok = q0 + mine / grp, head = kvh * grp + mine % grp;
+    float coef;
+    {
+      uint32_t raw[HD / 2];
+      const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (long)tok * a.ldq + (long)head * HD);
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const uint4 u = p[k];
+        raw[4 * k] = u.x; raw[4 * k + 1] = u.y; raw[4 * k + 2] = u.z; raw[4 * k + 3] = u.w;
+      }
+      const auto element = [&](int k) -> float {
+        const uint32_t u = raw[k / 2];
+        if (DT == QL_F16) return k & 1 ? __high2float(u32_as_h2(u)) : __low2float(u32_as_h2(u));
+        return __int_as_float(k & 1 ? u & 0xffff0000u : u << 16);
+      };
+      float mx = 0.f;
+#pragma unroll
+      for (int k = 0; k < HD; ++k) mx = fmaxf(mx, fabsf(element(k)));
+      const int e = stage_exponent(mx);
+      const float inv = copysignf(exp2i(-e), a.scale);
+      coef = exp2i(e) * (fabsf(a.scale) * 1.4426950408889634f);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        uint32_t h[4];                            // the order that the nibble masks give: (j, j + 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = h2_as_u32(__floats2half2_rn(element(8 * w + j) * inv, element(8 * w + j + 4) * inv));
+        *reinterpret_cast<uint4*>(smem + L::kQ + tile * L::kTile + panel_of<HD>(w) * L::kPanel + row * 128 +
+                                  ((column_of<HD>(w) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    }
+    ptx::fence_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(q_full);
+    const int pos = seq - ql + mine / grp;
+    const int row_lo = a.window ? max(pos - a.window + 1, 0) : 0, row_hi = pos + 1;
+    // steps where every row of the warp sees every position
+    const int warp_lo = __reduce_max_sync(0xffffffffu, row_lo), warp_hi = __reduce_min_sync(0xffffffffu, row_hi);
+    const uint32_t s_col = tmem + 256u * tile + ((uint32_t)(warp & 3) << 21), o_col = s_col + 128u;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < steps; ++j) {
+      if (!ptx::mbar_wait(s_full(tile), j & 1, const_cast<volatile int*>(abort_flag))) {
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      const int p0 = blk0 * kBlock + j * kStep;
+      const bool masked = p0 < warp_lo || p0 + kStep > warp_hi;
+      const int lo = row_lo - p0, hi = row_hi - p0;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kStep / 32; ++k) {
+        uint32_t v[32];
+        ptx::tmem_ld32(s_col + 32u * k, v);
+        ptx::tmem_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (32 * k + q >= lo && 32 * k + q < hi) mx = fmaxf(mx, __uint_as_float(v[q]));
+        } else {
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int q = 0; q < 32; ++q) m4[q & 3] = fmaxf(m4[q & 3], __uint_as_float(v[q]));
+          mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+        }
+      }
+      const float mn = mx == -INFINITY ? -INFINITY : mx * coef;
+      if (__any_sync(0xffffffffu, mn > m + kLazy)) {
+        const float top = fmaxf(m, mn), f = top > m ? ex2(m - top) : 1.f;
+        m = top;
+        l *= f;
+        if (j > 0) {                              // the product of the step before is complete
+#pragma unroll
+          for (int k = 0; k < HD / 32; ++k) {
+            uint32_t v[32];
+            ptx::tmem_ld32(o_col + 32u * k, v);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] = __float_as_uint(__uint_as_float(v[q]) * f);
+            ptx::tmem_st32(o_col + 32u * k, v);
+          }
+        }
+      }
+      const float base = kPShift - (m == -INFINITY ? 0.f : m);
+      float sum[4] = {};
+#pragma unroll
+      for (int k = 0; k < kStep / 32; ++k) {
+        uint32_t v[32], h[16];
+        ptx::tmem_ld32(s_col + 32u * k, v);
+        ptx::tmem_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 32; q += 2) {
+          float e0 = ex2(fmaf(__uint_as_float(v[q]), coef, base)), e1 = ex2(fmaf(__uint_as_float(v[q + 1]), coef, base));
+          if (masked) {
+            if (32 * k + q < lo || 32 * k + q >= hi) e0 = 0.f;
+            if (32 * k + q + 1 < lo || 32 * k + q + 1 >= hi) e1 = 0.f;
+          }
+          sum[(q >> 1) & 3] += e0 + e1;
+          h[q / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
+        }
+        ptx::tmem_st16(s_col + 16u * k, h);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(p_full(tile));
+    }
+    if (steps > 0 && ok) ok = ptx::mbar_wait(done, 0, const_cast<volatile int*>(abort_flag));
+    ptx::tc_fence_after();
+    if (*bad_flag || !ok) l = __int_as_float(0x7fc00000);
+    const float inv = l == 0.f ? 0.f : 1.f / l;   // a row that sees nothing is zero
+    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + ((long)tok * a.NH + head) * HD;
+#pragma unroll
+    for (int k = 0; k < HD / 32; ++k) {
+      uint32_t v[32];
+      if (steps > 0) {
+        ptx::tmem_ld32(o_col + 32u * k, v);
+        ptx::tmem_wait_ld();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {               // columns 8 (4 k + c) ...: one word's elements
+        const int pc = 4 * k + c, panel = pc >> 3, col = pc & 7;
+        const int w = HD == 64 ? pc : 4 * (col >> 1) + 2 * panel + (col & 1);
+        uint32_t o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          // element e of the word is at 2 e, elements 4 + e at 2 e + 1
+          const int e0 = 2 * q, e1 = 2 * q + 1;
+          const float y0 = steps > 0 ? __uint_as_float(v[8 * c + (e0 < 4 ? 2 * e0 : 2 * (e0 - 4) + 1)]) * inv : 0.f * inv;
+          const float y1 = steps > 0 ? __uint_as_float(v[8 * c + (e1 < 4 ? 2 * e1 : 2 * (e1 - 4) + 1)]) * inv : 0.f * inv;
+          if (DT == QL_F16) {
+            o[q] = h2_as_u32(__floats2half2_rn(y0, y1));
+          } else {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(y0, y1);
+            o[q] = *reinterpret_cast<const uint32_t*>(&t);
+          }
+        }
+        if (live) {
+          uint2* to = reinterpret_cast<uint2*>(out + 8 * w);
+          to[0] = make_uint2(o[0], o[1]);
+          to[1] = make_uint2(o[2], o[3]);
+        }
+      }
+    }
+  } else if (warp < kSoftWarps + kDecodeWarps) {
+    // ---------------- keys and values: warp d decodes blocks d, d + 4 of each step's 8
+    const int d = warp - kSoftWarps;
+    const uint32_t ring = sbase + L::kRaw + d * kRing * BB, bar = bar0 + 8u * (14 + d * kRing);
+    const unsigned char* raw = smem + L::kRaw + d * kRing * BB;
+    constexpr int LP = HD / 32, PW = 32 / LP;     // lanes of a position, positions of a pass
+    const int t = lane % LP, pr = lane / LP;
+    // the warp's blocks in order: n-th is block d + 4 n of the item. Lane i looks up block i of the next 32.
+    const int mine = nblk > d ? (nblk - d + 3) / 4 : 0;
+    const auto lookup = [&](int n) { return n < mine ? source(a, b, kvh, blk0, d + 4 * n, nblk) : kNoBlock; };
+    uint32_t src = lookup(lane), next = kNoBlock;
+    int issued = 0;
+    const auto issue_one = [&](int ahead_of) {     // block `issued`, whose lookup is in src or next
+      if (issued < mine && (issued & 31) == lane) {
+        const uint32_t at = (issued ^ ahead_of) & 32 ? next : src;
+        const int s = issued % kRing;
+        issue<BB>(a, at, s, ring, bar);
+      }
+      ++issued;
+    };
+    for (int k = 0; k < kRing; ++k) issue_one(0);
+    uint32_t missing = __ballot_sync(0xffffffffu, src == kNoBlock);
+    bool ok = true;
+    int n = 0;                                    // blocks decoded
+    for (int j = 0; ok && j < steps; ++j) {
+      const int st = j & 1, par = (j >> 1) & 1;
+      // both of this step's blocks arrive, keys first
+#pragma unroll
+      for (int kv = 0; kv < 2 && ok; ++kv) {
+        if (!ptx::mbar_wait(kv ? v_free(st) : k_free(st), par ^ 1, const_cast<volatile int*>(abort_flag))) {
+          ok = false;
+          break;
+        }
+        unsigned char* to = smem + (kv ? L::kV : L::kK) + st * L::kTile;
+        for (int half = 0; half < 2; ++half) {
+          const int bn = 2 * j + half;             // this warp's block, d + 4 bn of the item
+          bool have = bn < mine;
+          if (have && kv == 0) {
+            if ((bn & 31) == 0) {
+              if (bn > 0) {
+                src = next;
+                missing = __ballot_sync(0xffffffffu, src == kNoBlock);
+              }
+              next = lookup(bn + 32 + lane);
+            }
+            if (!ptx::mbar_wait(bar + 8 * (bn % kRing), (bn / kRing) & 1, const_cast<volatile int*>(abort_flag))) {
+              ok = false;
+              break;
+            }
+          }
+          if (have && ((missing >> (bn & 31)) & 1)) {
+            have = false;
+            if (lane == 0) *bad_flag = 1;          // a page that is not one of the cache's: nan
+          }
+          const unsigned char* blk = raw + (bn % kRing) * BB + (kv ? code_bytes(HD) + scale_bytes(HD, G) : 0);
+#pragma unroll
+          for (int pass = 0; pass < kBlock / PW; ++pass) {
+            const int p = pass * PW + pr, at = (2 * 4 * j + d + 4 * half) * kBlock + p;   // in the block, in the item
+            const int row = (d + 4 * half) * kBlock + p;
+            const int seen = blk0 * kBlock + at;
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            __half2 sm = h2_const(0u);
+            // positions that no row sees are zero: their memory may never have been written
+            if (have && seen >= lo_all && seen < hi_all) {
+              u = *reinterpret_cast<const uint4*>(blk + p * (HD / 2) + t * 16);
+              sm = reinterpret_cast<const __half2*>(blk + code_bytes(HD))[p * (HD / G) + t * 32 / G];
+            }
+            const __half2 s2 = __low2half2(sm), m2 = __high2half2(sm);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              __half2 h[4];
+              codes_h2(w[i], h);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) h[q] = __hfma2(h[q], s2, m2);
+              const int word = 4 * t + i;
+              *reinterpret_cast<uint4*>(to + panel_of<HD>(word) * L::kPanel + row * 128 +
+                                        ((column_of<HD>(word) ^ (row & 7)) << 4)) =
+                  make_uint4(h2_as_u32(h[0]), h2_as_u32(h[1]), h2_as_u32(h[2]), h2_as_u32(h[3]));
+            }
+          }
+          if (kv == 1 && bn < mine) {              // the block's values were its last part
+            __syncwarp();
+            ++n;
+            issue_one(bn);
+          }
+        }
+        ptx::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(kv ? v_full(st) : k_full(st));
+      }
+    }
+    if (!ok)                                       // no copy is left in flight
+      for (int k = n; k < min(issued, mine); ++k) ptx::mbar_wait_drain(bar + 8 * (k % kRing), (k / kRing) & 1);
+  } else if (lane == 0 && steps > 0) {
+    // ---------------- MMA issue
+    constexpr uint32_t kIdescS = ptx::idesc_f16_f32(128, kStep);
+    constexpr uint32_t kIdescO = ptx::idesc_f16_f32(128, HD) | ptx::kIdescBMn;
+    volatile int* ab = const_cast<volatile int*>(abort_flag);
+    const auto scores = [&](int i, int st) {
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        const uint32_t at = (k >> 2) * L::kPanel + (k & 3) * 32;
+        ptx::mma_f16_ss(tmem + 256u * i, ptx::smem_desc_sw128(sbase + L::kQ + i * L::kTile + at),
+                        ptx::smem_desc_sw128(sbase + L::kK + st * L::kTile + at), kIdescS, k > 0);
+      }
+      ptx::mma_commit(s_full(i));
+    };
+    bool ok = ptx::mbar_wait(q_full, 0, ab) && ptx::mbar_wait(k_full(0), 0, ab);
+    ptx::tc_fence_after();
+    if (ok) {
+      scores(0, 0);
+      scores(1, 0);
+      ptx::mma_commit(k_free(0));
+    }
+    for (int j = 0; ok && j < steps; ++j) {
+      const int st = j & 1, par = (j >> 1) & 1, st1 = st ^ 1, par1 = ((j + 1) >> 1) & 1;
+      for (int i = 0; i < kTiles; ++i) {
+        if (!ptx::mbar_wait(p_full(i), j & 1, ab) || (i == 0 && !ptx::mbar_wait(v_full(st), par, ab)) ||
+            (i == 0 && j + 1 < steps && !ptx::mbar_wait(k_full(st1), par1, ab))) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kStep / 16; ++k)
+          ptx::mma_f16_ts(tmem + 256u * i + 128u, tmem + 256u * i + 8u * k,
+                          ptx::smem_desc_mn_sw128(sbase + L::kV + st * L::kTile + k * 2048, L::kPanel), kIdescO,
+                          j > 0 || k > 0);
+        if (j + 1 < steps) scores(i, st1);
+      }
+      if (!ok) break;
+      ptx::mma_commit(v_free(st));
+      if (j + 1 < steps) ptx::mma_commit(k_free(st1));
+    }
+    // everything issued has completed before tensor memory is read for the output or released
+    ptx::mma_commit(done);
+    ptx::mbar_wait_drain(done, 0);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_kv4_prompt_status, 1);
+  if (warp == kWarps - 1) ptx::tmem_dealloc(tmem, 512);
+}
+
+template <int DT, int HD, int G>
+int launch(const AttnArgs& a, cudaStream_t st) {
+  auto kern = kv4_prompt_kernel<DT, HD, G>;
+  static int configured_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_dev != dev) {
+    const int rc = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, G>::kBytes),
+                               "cudaFuncSetAttribute(kv4 prompt smem)");
+    if (rc) return rc;
+    configured_dev = dev;
+  }
+  const long pairs = (long)a.T * (a.NH / a.NKV) / (kTiles * kTileRows) + a.B;
+  kern<<<(unsigned)(pairs * a.NKV), kThreads, Smem<HD, G>::kBytes, st>>>(a);
+  return cuda_status(cudaGetLastError(), "ql_kv4_attention (prompt) launch");
+}
+
+template <int DT>
+int launch_sizes(const AttnArgs& a, int HD, int group, cudaStream_t st) {
+  if (HD == 64) return group == 32 ? launch<DT, 64, 32>(a, st) : launch<DT, 64, 64>(a, st);
+  return group == 32   ? launch<DT, 128, 32>(a, st)
+         : group == 64 ? launch<DT, 128, 64>(a, st)
+                       : launch<DT, 128, 128>(a, st);
+}
+
+}  // namespace
+
+int kv4_prompt_attention(const AttnArgs& a, int dtype, int HD, int group, cudaStream_t st) {
+  return dtype == QL_F16 ? launch_sizes<QL_F16>(a, HD, group, st) : launch_sizes<QL_BF16>(a, HD, group, st);
+}
+
+int take_kv4_prompt_status() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_kv4_prompt_status, sizeof(int)) != cudaSuccess) return 0;
+  if (v) cudaMemcpyToSymbol(g_kv4_prompt_status, &zero, sizeof(int));
+  return v;
+}
+
+}  // namespace ql
