@@ -4,9 +4,11 @@
 //
 // A CTA takes two tiles of 128 rows of one request and key/value head and walks the positions they see
 // in steps of 128:
-//   S = Q K^T  (tcgen05, 128 x 128, Q and K in shared memory)      softmax  P = 2^(coef S - m)
+//   S = Q K^T  (tcgen05, Q and K in shared memory)      softmax  P = 2^(coef S - m)
 //   O = O + P V  (P from tensor memory, where it takes the place of S; V in shared memory)
-// The tiles alternate, so the tensor cores work on one while the other is in its softmax. Warps 0 - 3 and
+// The softmax takes a step in two halves of 64 columns. As soon as it has written P of one, its product and
+// then S of the same half of the next step are issued, which finish while it works on the other: it never
+// waits for the tensor cores in the steady state. Warps 0 - 3 and
 // 4 - 7 are the tiles' softmax, a thread a row; warps 8 - 11 decode keys and values, once for both tiles;
 // warp 12 issues the MMAs. The running maximum moves only when it grows by more than 2^kLazy, and
 // then the row's O in tensor memory is scaled.
@@ -28,7 +30,7 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kTileRows = 128, kTiles = 2, kStep = 128;
+constexpr int kTileRows = 128, kTiles = 2, kStep = 128, kHalf = kStep / 2;
 constexpr int kSoftWarps = 8, kDecodeWarps = 4, kWarps = kSoftWarps + kDecodeWarps + 1, kThreads = kWarps * 32;
 constexpr int kRing = 3;                        // blocks of a decoding warp in flight
 
@@ -41,8 +43,9 @@ struct Smem {
   static constexpr int kV = kK + 2 * kTile;
   static constexpr int kRaw = kV + 2 * kTile;
   static constexpr int kBar = kRaw + kDecodeWarps * kRing * block_bytes(HD, G);
-  // s_full[2], p_full[2], k_full[2], v_full[2], k_free[2], v_free[2], q_full, done, ring[4][3]
-  static constexpr int kBars = 14 + kDecodeWarps * kRing;
+  // s_full[2][2], p_full[2][2], k_full[2], v_full[2], k_free[2], v_free[2], pv_done[2], q_full, done, ring[4][3]
+  static constexpr int kRingBar = 20;
+  static constexpr int kBars = kRingBar + kDecodeWarps * kRing;
   static constexpr int kMisc = kBar + kBars * 8;
   static constexpr int kBytes = kMisc + 16 + 1024;   // + alignment slack
 };
@@ -59,11 +62,109 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Pairs of fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+constexpr float kLazy = 6.f, kPShift = 9.f;      // as in the streaming kernel
+
+// A row's running maximum (units of log2) and sum.
+struct Row {
+  float m, l;
+};
+
+// Half a step of a row: S in tensor memory to P over it. lo / hi: the positions that the row sees, relative to
+// the half; product: the barrier and parity of the product before this one, which has to be complete before
+// O is scaled; MASKED: they are not all of them for every row of the warp. The next 16 columns are loaded
+// while the last are worked on.
+template <int HD, bool MASKED>
+__device__ __forceinline__ bool softmax_half(Row& row, uint32_t s_col, uint32_t o_col, float coef, bool first, int lo,
+                                             int hi, uint32_t product, uint32_t parity, volatile int* abort_flag) {
+  constexpr int NC = kHalf / 16;
+  uint32_t v[2][16];
+  float mx = -INFINITY;
+  ptx::tmem_ld16(s_col, v[0]);
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    ptx::tmem_wait_ld();
+    if (k + 1 < NC) ptx::tmem_ld16(s_col + 16u * (k + 1), v[(k + 1) & 1]);
+    float m2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int q = 0; q < 16; q += 2) {
+      float x = __uint_as_float(v[k & 1][q]), y = __uint_as_float(v[k & 1][q + 1]);
+      if (MASKED) {
+        if (16 * k + q < lo || 16 * k + q >= hi) x = -INFINITY;
+        if (16 * k + q + 1 < lo || 16 * k + q + 1 >= hi) y = -INFINITY;
+      }
+      m2[(q >> 1) & 1] = fmaxf(m2[(q >> 1) & 1], fmaxf(x, y));
+    }
+    mx = fmaxf(mx, fmaxf(m2[0], m2[1]));
+  }
+  const float mn = MASKED && mx == -INFINITY ? -INFINITY : mx * coef;   // coef may be 0
+  if (__any_sync(0xffffffffu, mn > row.m + kLazy)) {
+    const float top = fmaxf(row.m, mn), f = top > row.m ? ex2(row.m - top) : 1.f;
+    row.m = top;
+    row.l *= f;
+    if (!first) {
+      if (!ptx::mbar_wait(product, parity, abort_flag)) return false;
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        uint32_t o[16];
+        ptx::tmem_ld16(o_col + 16u * k, o);
+        ptx::tmem_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+        ptx::tmem_st16(o_col + 16u * k, o);
+      }
+    }
+  }
+  const float base = kPShift - (MASKED && row.m == -INFINITY ? 0.f : row.m);
+  const float2 coef2 = make_float2(coef, coef), base2 = make_float2(base, base);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  ptx::tmem_ld16(s_col, v[0]);
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    ptx::tmem_wait_ld();
+    if (k + 1 < NC) ptx::tmem_ld16(s_col + 16u * (k + 1), v[(k + 1) & 1]);
+    uint32_t h[8];
+#pragma unroll
+    for (int q = 0; q < 16; q += 2) {
+      float2 e = fma2(make_float2(__uint_as_float(v[k & 1][q]), __uint_as_float(v[k & 1][q + 1])), coef2, base2);
+      e = make_float2(ex2(e.x), ex2(e.y));
+      if (MASKED) {
+        if (16 * k + q < lo || 16 * k + q >= hi) e.x = 0.f;
+        if (16 * k + q + 1 < lo || 16 * k + q + 1 >= hi) e.y = 0.f;
+      }
+      sum[(q >> 1) & 1] = add2(sum[(q >> 1) & 1], e);
+      h[q / 2] = h2_as_u32(__floats2half2_rn(e.x, e.y));
+    }
+    ptx::tmem_st8(s_col + 8u * k, h);
+  }
+  sum[0] = add2(sum[0], sum[1]);
+  row.l += sum[0].x + sum[0].y;
+  ptx::tmem_wait_st();
+  return true;
+}
+
 template <int DT, int HD, int G>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
   using L = Smem<HD, G>;
   constexpr int BB = block_bytes(HD, G), W = HD / 8;
-  constexpr float kLazy = 6.f, kPShift = 9.f;
   const int grp = a.NH / a.NKV;
   // tiles of the longest rows first
   const int kvh = blockIdx.x % a.NKV, x = gridDim.x / a.NKV - 1 - blockIdx.x / a.NKV;
@@ -87,21 +188,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = ptx::smem_addr(smem), bar0 = sbase + L::kBar;
-  const auto s_full = [&](int i) { return bar0 + 8u * i; };
-  const auto p_full = [&](int i) { return bar0 + 8u * (2 + i); };
-  const auto k_full = [&](int s) { return bar0 + 8u * (4 + s); };
-  const auto v_full = [&](int s) { return bar0 + 8u * (6 + s); };
-  const auto k_free = [&](int s) { return bar0 + 8u * (8 + s); };
-  const auto v_free = [&](int s) { return bar0 + 8u * (10 + s); };
-  const uint32_t q_full = bar0 + 8u * 12, done = bar0 + 8u * 13;
+  const auto s_full = [&](int i, int h) { return bar0 + 8u * (2 * i + h); };
+  const auto p_full = [&](int i, int h) { return bar0 + 8u * (4 + 2 * i + h); };
+  const auto k_full = [&](int s) { return bar0 + 8u * (8 + s); };
+  const auto v_full = [&](int s) { return bar0 + 8u * (10 + s); };
+  const auto k_free = [&](int s) { return bar0 + 8u * (12 + s); };
+  const auto v_free = [&](int s) { return bar0 + 8u * (14 + s); };
+  const auto pv_done = [&](int i) { return bar0 + 8u * (16 + i); };
+  const uint32_t q_full = bar0 + 8u * 18, done = bar0 + 8u * 19;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
   volatile int* bad_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 8);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // uniform
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(s_full(i), 1);
-      ptx::mbar_init(p_full(i), 4);
+      for (int h = 0; h < 2; ++h) {
+        ptx::mbar_init(s_full(i, h), 1);
+        ptx::mbar_init(p_full(i, h), 4);
+      }
+      ptx::mbar_init(pv_done(i), 1);
       ptx::mbar_init(k_full(i), kDecodeWarps);
       ptx::mbar_init(v_full(i), kDecodeWarps);
       ptx::mbar_init(k_free(i), 1);
@@ -109,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     }
     ptx::mbar_init(q_full, kSoftWarps);
     ptx::mbar_init(done, 1);
-    for (int i = 0; i < kDecodeWarps * kRing; ++i) ptx::mbar_init(bar0 + 8u * (14 + i), 1);
+    for (int i = 0; i < kDecodeWarps * kRing; ++i) ptx::mbar_init(bar0 + 8u * (L::kRingBar + i), 1);
     *abort_flag = 0;
     *bad_flag = seq > table_end;                  // a length past the table: nan
     ptx::fence_mbar_init();
@@ -121,7 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = 0u;                       // all 512 columns are this CTA's
+  if (threadIdx.x == 0 && *tmem_slot != 0u) *abort_flag = 1;
   // tensor memory of tile i: S (and P over it) at 256 i, O at 256 i + 128
 
   if (warp < kSoftWarps) {
@@ -167,80 +273,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     // steps where every row of the warp sees every position
     const int warp_lo = __reduce_max_sync(0xffffffffu, row_lo), warp_hi = __reduce_min_sync(0xffffffffu, row_hi);
     const uint32_t s_col = tmem + 256u * tile + ((uint32_t)(warp & 3) << 21), o_col = s_col + 128u;
-    float m = -INFINITY, l = 0.f;
+    Row run = {-INFINITY, 0.f};
     bool ok = true;
-    for (int j = 0; j < steps; ++j) {
-      if (!ptx::mbar_wait(s_full(tile), j & 1, const_cast<volatile int*>(abort_flag))) {
-        ok = false;
-        break;
-      }
-      ptx::tc_fence_after();
-      const int p0 = blk0 * kBlock + j * kStep;
-      const bool masked = p0 < warp_lo || p0 + kStep > warp_hi;
-      const int lo = row_lo - p0, hi = row_hi - p0;
-      float mx = -INFINITY;
+    volatile int* ab = const_cast<volatile int*>(abort_flag);
+    for (int j = 0; ok && j < steps; ++j) {
 #pragma unroll
-      for (int k = 0; k < kStep / 32; ++k) {
-        uint32_t v[32];
-        ptx::tmem_ld32(s_col + 32u * k, v);
-        ptx::tmem_wait_ld();
-        if (masked) {
-#pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (32 * k + q >= lo && 32 * k + q < hi) mx = fmaxf(mx, __uint_as_float(v[q]));
-        } else {
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int q = 0; q < 32; ++q) m4[q & 3] = fmaxf(m4[q & 3], __uint_as_float(v[q]));
-          mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+      for (int h = 0; h < 2; ++h) {
+        ok = ok && ptx::mbar_wait(s_full(tile, h), j & 1, ab);
+        ptx::tc_fence_after();
+        const int p0 = blk0 * kBlock + j * kStep + h * kHalf, n = 2 * j + h;
+        const bool masked = p0 < warp_lo || p0 + kHalf > warp_hi;
+        if (__any_sync(0xffffffffu, !ok)) {
+          ok = false;
+          break;
         }
+        if (masked)
+          ok = softmax_half<HD, true>(run, s_col + h * kHalf, o_col, coef, n == 0, row_lo - p0, row_hi - p0, pv_done(tile),
+                                      (n & 1) ^ 1, ab);
+        else
+          ok = softmax_half<HD, false>(run, s_col + h * kHalf, o_col, coef, n == 0, 0, kHalf, pv_done(tile), (n & 1) ^ 1, ab);
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_full(tile, h));
       }
-      const float mn = mx == -INFINITY ? -INFINITY : mx * coef;
-      if (__any_sync(0xffffffffu, mn > m + kLazy)) {
-        const float top = fmaxf(m, mn), f = top > m ? ex2(m - top) : 1.f;
-        m = top;
-        l *= f;
-        if (j > 0) {                              // the product of the step before is complete
-#pragma unroll
-          for (int k = 0; k < HD / 32; ++k) {
-            uint32_t v[32];
-            ptx::tmem_ld32(o_col + 32u * k, v);
-            ptx::tmem_wait_ld();
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = __float_as_uint(__uint_as_float(v[q]) * f);
-            ptx::tmem_st32(o_col + 32u * k, v);
-          }
-        }
-      }
-      const float base = kPShift - (m == -INFINITY ? 0.f : m);
-      float sum[4] = {};
-#pragma unroll
-      for (int k = 0; k < kStep / 32; ++k) {
-        uint32_t v[32], h[16];
-        ptx::tmem_ld32(s_col + 32u * k, v);
-        ptx::tmem_wait_ld();
-#pragma unroll
-        for (int q = 0; q < 32; q += 2) {
-          float e0 = ex2(fmaf(__uint_as_float(v[q]), coef, base)), e1 = ex2(fmaf(__uint_as_float(v[q + 1]), coef, base));
-          if (masked) {
-            if (32 * k + q < lo || 32 * k + q >= hi) e0 = 0.f;
-            if (32 * k + q + 1 < lo || 32 * k + q + 1 >= hi) e1 = 0.f;
-          }
-          sum[(q >> 1) & 3] += e0 + e1;
-          h[q / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
-        }
-        ptx::tmem_st16(s_col + 16u * k, h);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      ptx::tmem_wait_st();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(p_full(tile));
     }
     if (steps > 0 && ok) ok = ptx::mbar_wait(done, 0, const_cast<volatile int*>(abort_flag));
     ptx::tc_fence_after();
-    if (*bad_flag || !ok) l = __int_as_float(0x7fc00000);
-    const float inv = l == 0.f ? 0.f : 1.f / l;   // a row that sees nothing is zero
+    if (*bad_flag || !ok) run.l = __int_as_float(0x7fc00000);
+    const float inv = run.l == 0.f ? 0.f : 1.f / run.l;   // a row that sees nothing is zero
     uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + ((long)tok * a.NH + head) * HD;
 #pragma unroll
     for (int k = 0; k < HD / 32; ++k) {
@@ -277,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
   } else if (warp < kSoftWarps + kDecodeWarps) {
     // ---------------- keys and values: warp d decodes blocks d, d + 4 of each step's 8
     const int d = warp - kSoftWarps;
-    const uint32_t ring = sbase + L::kRaw + d * kRing * BB, bar = bar0 + 8u * (14 + d * kRing);
+    const uint32_t ring = sbase + L::kRaw + d * kRing * BB, bar = bar0 + 8u * (L::kRingBar + d * kRing);
     const unsigned char* raw = smem + L::kRaw + d * kRing * BB;
     constexpr int LP = HD / 32, PW = 32 / LP;     // lanes of a position, positions of a pass
     const int t = lane % LP, pr = lane / LP;
@@ -303,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
       // both of this step's blocks arrive, keys first
 #pragma unroll
       for (int kv = 0; kv < 2 && ok; ++kv) {
-        if (!ptx::mbar_wait(kv ? v_free(st) : k_free(st), par ^ 1, const_cast<volatile int*>(abort_flag))) {
+        if (!ptx::mbar_wait_sleep(kv ? v_free(st) : k_free(st), par ^ 1, const_cast<volatile int*>(abort_flag))) {
           ok = false;
           break;
         }
@@ -368,49 +428,74 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     }
     if (!ok)                                       // no copy is left in flight
       for (int k = n; k < min(issued, mine); ++k) ptx::mbar_wait_drain(bar + 8 * (k % kRing), (k / kRing) & 1);
-  } else if (lane == 0 && steps > 0) {
-    // ---------------- MMA issue
-    constexpr uint32_t kIdescS = ptx::idesc_f16_f32(128, kStep);
+  } else if (steps > 0) {
+    // ---------------- MMA issue: the warp runs converged, one lane issues, and what the MMAs take is the
+    // same for all lanes by construction (tensor memory is all this CTA's, so it begins at 0), which keeps
+    // descriptors in uniform registers: about 110 cycles an MMA without, against 64 of tensor work
+    constexpr uint32_t kIdescS = ptx::idesc_f16_f32(128, kHalf);
     constexpr uint32_t kIdescO = ptx::idesc_f16_f32(128, HD) | ptx::kIdescBMn;
     volatile int* ab = const_cast<volatile int*>(abort_flag);
-    const auto scores = [&](int i, int st) {
+    const uint64_t q_desc = ptx::smem_desc_sw128(sbase + L::kQ), k_desc = ptx::smem_desc_sw128(sbase + L::kK);
+    const uint64_t v_desc = ptx::smem_desc_mn_sw128(sbase + L::kV, L::kPanel);
+    const bool elected = ptx::elect_one();
+    const auto scores = [&](int i, int h, int st) {
+      const uint64_t qd = q_desc + (uint32_t)(i * (L::kTile >> 4));
+      const uint64_t kd = k_desc + (uint32_t)((st * L::kTile + h * kHalf * 128) >> 4);
+      if (elected) {
 #pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        const uint32_t at = (k >> 2) * L::kPanel + (k & 3) * 32;
-        ptx::mma_f16_ss(tmem + 256u * i, ptx::smem_desc_sw128(sbase + L::kQ + i * L::kTile + at),
-                        ptx::smem_desc_sw128(sbase + L::kK + st * L::kTile + at), kIdescS, k > 0);
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t at = ((k >> 2) * L::kPanel + (k & 3) * 32) >> 4;
+          ptx::mma_f16_ss(256u * i + (uint32_t)(h * kHalf), qd + at, kd + at, kIdescS, k > 0);
+        }
+        ptx::mma_commit(s_full(i, h));
       }
-      ptx::mma_commit(s_full(i));
+      __syncwarp();
     };
     bool ok = ptx::mbar_wait(q_full, 0, ab) && ptx::mbar_wait(k_full(0), 0, ab);
+    ok = __all_sync(0xffffffffu, ok);
     ptx::tc_fence_after();
     if (ok) {
-      scores(0, 0);
-      scores(1, 0);
-      ptx::mma_commit(k_free(0));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        scores(0, h, 0);
+        scores(1, h, 0);
+      }
+      if (elected) ptx::mma_commit(k_free(0));
     }
     for (int j = 0; ok && j < steps; ++j) {
       const int st = j & 1, par = (j >> 1) & 1, st1 = st ^ 1, par1 = ((j + 1) >> 1) & 1;
-      for (int i = 0; i < kTiles; ++i) {
-        if (!ptx::mbar_wait(p_full(i), j & 1, ab) || (i == 0 && !ptx::mbar_wait(v_full(st), par, ab)) ||
-            (i == 0 && j + 1 < steps && !ptx::mbar_wait(k_full(st1), par1, ab))) {
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < kStep / 16; ++k)
-          ptx::mma_f16_ts(tmem + 256u * i + 128u, tmem + 256u * i + 8u * k,
-                          ptx::smem_desc_mn_sw128(sbase + L::kV + st * L::kTile + k * 2048, L::kPanel), kIdescO,
-                          j > 0 || k > 0);
-        if (j + 1 < steps) scores(i, st1);
+      for (int hi = 0; hi < 2 * kTiles; ++hi) {
+        const int h = hi >> 1, i = hi & 1;
+        bool go = ptx::mbar_wait(p_full(i, h), j & 1, ab);
+        if (hi == 0) {
+          go = go && ptx::mbar_wait(v_full(st), par, ab);
+          if (j + 1 < steps) go = go && ptx::mbar_wait(k_full(st1), par1, ab);
+        }
+        ok = ok && __all_sync(0xffffffffu, go);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint64_t vd = v_desc + (uint32_t)((st * L::kTile + h * kHalf * 128) >> 4);
+        if (elected) {
+#pragma unroll
+          for (int k = 0; k < kHalf / 16; ++k)
+            ptx::mma_f16_ts_elected(256u * i + 128u, 256u * i + (uint32_t)(h * kHalf) + 8u * k,
+                                    vd + (uint32_t)(k * (2048 >> 4)), kIdescO, h > 0 || k > 0 || j > 0);
+          ptx::mma_commit(pv_done(i));
+        }
+        __syncwarp();
+        if (j + 1 < steps) scores(i, h, st1);
       }
       if (!ok) break;
-      ptx::mma_commit(v_free(st));
-      if (j + 1 < steps) ptx::mma_commit(k_free(st1));
+      if (elected) {
+        ptx::mma_commit(v_free(st));
+        if (j + 1 < steps) ptx::mma_commit(k_free(st1));
+      }
+      __syncwarp();
     }
     // everything issued has completed before tensor memory is read for the output or released
-    ptx::mma_commit(done);
+    if (elected) ptx::mma_commit(done);
+    __syncwarp();
     ptx::mbar_wait_drain(done, 0);
   }
   ptx::tc_fence_before();
