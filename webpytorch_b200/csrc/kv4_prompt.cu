@@ -62,6 +62,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// A wait by a whole warp. The lanes leave the polling loop at different times, and the tensor-memory
+// instructions that follow want the warp converged: the vote brings it together, and the answer is the same
+// for all lanes.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag));
+}
+
 // Pairs of fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -120,7 +127,7 @@ __device__ __forceinline__ bool softmax_half(Row& row, uint32_t s_col, uint32_t 
     row.m = top;
     row.l *= f;
     if (!first) {
-      if (!ptx::mbar_wait(product, parity, abort_flag)) return false;
+      if (!warp_wait(product, parity, abort_flag)) return false;
       ptx::tc_fence_after();
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
@@ -226,9 +233,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = 0u;                       // all 512 columns are this CTA's
-  if (threadIdx.x == 0 && *tmem_slot != 0u) *abort_flag = 1;
-  // tensor memory of tile i: S (and P over it) at 256 i, O at 256 i + 128
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);   // known to be the same for all lanes
+  // tensor memory of tile i: S (and P over it) at tmem + 256 i, O 128 columns on
 
   if (warp < kSoftWarps) {
     // ---------------- softmax: a thread a row
@@ -279,25 +285,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     for (int j = 0; ok && j < steps; ++j) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        ok = ok && ptx::mbar_wait(s_full(tile, h), j & 1, ab);
+        ok = warp_wait(s_full(tile, h), j & 1, ab);
+        if (!ok) break;
         ptx::tc_fence_after();
         const int p0 = blk0 * kBlock + j * kStep + h * kHalf, n = 2 * j + h;
         const bool masked = p0 < warp_lo || p0 + kHalf > warp_hi;
-        if (__any_sync(0xffffffffu, !ok)) {
-          ok = false;
-          break;
-        }
         if (masked)
           ok = softmax_half<HD, true>(run, s_col + h * kHalf, o_col, coef, n == 0, row_lo - p0, row_hi - p0, pv_done(tile),
                                       (n & 1) ^ 1, ab);
         else
           ok = softmax_half<HD, false>(run, s_col + h * kHalf, o_col, coef, n == 0, 0, kHalf, pv_done(tile), (n & 1) ^ 1, ab);
+        if (!ok) break;
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_full(tile, h));
+        __syncwarp();
       }
     }
-    if (steps > 0 && ok) ok = ptx::mbar_wait(done, 0, const_cast<volatile int*>(abort_flag));
+    if (steps > 0 && ok) ok = warp_wait(done, 0, ab);
     ptx::tc_fence_after();
     if (*bad_flag || !ok) run.l = __int_as_float(0x7fc00000);
     const float inv = run.l == 0.f ? 0.f : 1.f / run.l;   // a row that sees nothing is zero
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
       for (int k = n; k < min(issued, mine); ++k) ptx::mbar_wait_drain(bar + 8 * (k % kRing), (k / kRing) & 1);
   } else if (steps > 0) {
     // ---------------- MMA issue: the warp runs converged, one lane issues, and what the MMAs take is the
-    // same for all lanes by construction (tensor memory is all this CTA's, so it begins at 0), which keeps
+    // same for all lanes by construction, which keeps
     // descriptors in uniform registers: about 110 cycles an MMA without, against 64 of tensor work
     constexpr uint32_t kIdescS = ptx::idesc_f16_f32(128, kHalf);
     constexpr uint32_t kIdescO = ptx::idesc_f16_f32(128, HD) | ptx::kIdescBMn;
@@ -445,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t at = ((k >> 2) * L::kPanel + (k & 3) * 32) >> 4;
-          ptx::mma_f16_ss(256u * i + (uint32_t)(h * kHalf), qd + at, kd + at, kIdescS, k > 0);
+          ptx::mma_f16_ss(tmem + 256u * i + (uint32_t)(h * kHalf), qd + at, kd + at, kIdescS, k > 0);
         }
         ptx::mma_commit(s_full(i, h));
       }
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
         if (elected) {
 #pragma unroll
           for (int k = 0; k < kHalf / 16; ++k)
-            ptx::mma_f16_ts_elected(256u * i + 128u, 256u * i + (uint32_t)(h * kHalf) + 8u * k,
+            ptx::mma_f16_ts_elected(tmem + 256u * i + 128u, tmem + 256u * i + (uint32_t)(h * kHalf) + 8u * k,
                                     vd + (uint32_t)(k * (2048 >> 4)), kIdescO, h > 0 || k > 0 || j > 0);
           ptx::mma_commit(pv_done(i));
         }
@@ -493,15 +498,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
       }
       __syncwarp();
     }
-    // everything issued has completed before tensor memory is read for the output or released
-    if (elected) ptx::mma_commit(done);
-    __syncwarp();
-    ptx::mbar_wait_drain(done, 0);
+    // everything issued has completed before tensor memory is read for the output or released. One lane polls, and
+    // the warp comes together before the end, which releases tensor memory once.
+    if (elected) {
+      ptx::mma_commit(done);
+      ptx::mbar_wait_drain(done, 0);
+    }
   }
+  __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_kv4_prompt_status, 1);
+  __syncwarp();
   if (warp == kWarps - 1) ptx::tmem_dealloc(tmem, 512);
 }
 
