@@ -16,7 +16,6 @@ A step of a batch:
 Every call is asynchronous on the current stream (or `stream`), without a host read of any length,
 so a step can be captured in a CUDA graph.
 """
-import math
 from collections import namedtuple
 
 import torch
@@ -30,12 +29,16 @@ Plan = namedtuple("Plan", "seq_lens cu_new slots positions requests n_free")
 
 
 def _need(t, name, dtype, dim):
+    """t is a GPU tensor of this type and number of dimensions, its last one contiguous."""
+    if type(t) is torch.Tensor and t.dtype is dtype and t.is_cuda and t.dim() == dim and (
+            t.is_contiguous() or t.stride(-1) == 1):
+        return                                     # the calls take a few microseconds: keep this short
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != dim:
         raise TypeError("%s must be a %d-D %s tensor, got %s" % (
             name, dim, dtype, "%s %s" % (t.dtype, tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t).__name__))
     if not t.is_cuda:
         raise ValueError("%s must be on the GPU" % name)
-    if dim and t.stride(-1) != 1 and t.shape[-1] > 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError("%s must be contiguous along its last dimension" % name)
 
 
@@ -65,8 +68,7 @@ class KV4Cache:
         """(k, v) fp16 [T, NKV, HD]: the values that slots int64 [T] stand for; zeros for -1."""
         _need(slots, "slots", torch.int64, 1)
         T = slots.shape[0]
-        k = torch.empty((T, self.NKV, self.HD), dtype=torch.float16, device=self.device)
-        v = torch.empty_like(k)
+        k, v = slots.new_empty((2, T, self.NKV, self.HD), dtype=torch.float16).unbind(0)
         _ffi.call("ql_kv4_read", self.data.data_ptr(), self.num_pages, self.NKV, self.HD, self.page, self.group,
                   slots.data_ptr(), T, k.data_ptr(), v.data_ptr(), _ffi.stream_ptr(stream, self.device))
         return k, v
@@ -78,7 +80,7 @@ _workspaces = {}
 def _attention_workspace(cache, NH, stream):
     """The attention's workspace on this stream, made once and shared by the layers' caches: its counters
     are zero between calls, and calls that share one may not overlap."""
-    key = (cache.device, cache.HD, _ffi.stream_ptr(stream, cache.device))
+    key = (cache.device.index, cache.HD, _ffi.stream_ptr(stream, cache.device))
     ws = _workspaces.get(key)
     if ws is None:
         if torch.cuda.is_current_stream_capturing():
@@ -104,20 +106,20 @@ def plan(prev_lens, new_lens, block_table, free_pages, n_free, page, max_tokens,
     _need(block_table, "block_table", torch.int32, 2)
     _need(free_pages, "free_pages", torch.int32, 1)
     _need(n_free, "n_free", torch.int32, 1)
-    n = prev_lens.shape[0]
-    if new_lens.shape[0] != n or block_table.shape[0] != n:
+    n, width = block_table.shape
+    if new_lens.shape[0] != n or prev_lens.shape[0] != n:
         raise ValueError("prev_lens, new_lens and block_table must have a row for each request: %d, %d, %d"
-                         % (n, new_lens.shape[0], block_table.shape[0]))
+                         % (prev_lens.shape[0], new_lens.shape[0], n))
     max_tokens = int(max_tokens)
-    dev = prev_lens.device
-    ws_bytes = int(_ffi.fn("ql_kv_plan_workspace")(n))
-    lens, cu, pos, req, left, ws = torch.empty(2 * n + 2 + 2 * max_tokens + ws_bytes // 4, dtype=torch.int32,
-                                               device=dev).split([n, n + 1, max_tokens, max_tokens, 1, ws_bytes // 4])
-    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
-    _ffi.call("ql_kv_plan", prev_lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(), block_table.stride(0),
-              block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], n_free.data_ptr(), page, max_tokens,
-              lens.data_ptr(), cu.data_ptr(), slots.data_ptr(), pos.data_ptr(), req.data_ptr(), left.data_ptr(),
-              ws.data_ptr(), ws_bytes, _ffi.stream_ptr(stream, dev))
+    ws_ints = int(_ffi.fn("ql_kv_plan_workspace")(n)) // 4
+    lens, cu, pos, req, left, ws = torch.unsafe_split_with_sizes(
+        prev_lens.new_empty(2 * n + 2 + 2 * max_tokens + ws_ints), (n, n + 1, max_tokens, max_tokens, 1, ws_ints))
+    slots = prev_lens.new_empty(max_tokens, dtype=torch.int64)
+    _ffi.call("ql_kv_plan", prev_lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(),
+              block_table.stride(0) if n > 1 else width, width, free_pages.data_ptr(), free_pages.shape[0],
+              n_free.data_ptr(), page, max_tokens, lens.data_ptr(), cu.data_ptr(), slots.data_ptr(), pos.data_ptr(),
+              req.data_ptr(), left.data_ptr(), ws.data_ptr() if ws_ints else None, 4 * ws_ints,
+              _ffi.stream_ptr(stream, prev_lens.device))
     return Plan(lens, cu, slots, pos, req, left)
 
 
@@ -128,37 +130,38 @@ def qk_norm_rope(qkv, NH, NKV, HD, positions, cos, sin, *, q_weight=None, k_weig
     [lmax, rot / 2]. With a cache, keys and values are quantised into its slots int64 [T] and (q, None)
     comes back, without one (q, k); q [T, NH, HD], k [T, NKV, HD] in qkv's dtype. A negative position is
     padding."""
-    if qkv.dim() != 2 or qkv.shape[1] != (NH + 2 * NKV) * HD:
-        raise ValueError("qkv must be [T, %d], got %s" % ((NH + 2 * NKV) * HD, tuple(qkv.shape)))
     _need(qkv, "qkv", qkv.dtype, 2)
-    T = qkv.shape[0]
+    T, width = qkv.shape
+    if width != (NH + 2 * NKV) * HD:
+        raise ValueError("qkv must be [T, %d], got %s" % ((NH + 2 * NKV) * HD, tuple(qkv.shape)))
     _need(positions, "positions", torch.int32, 1)
     _need(cos, "cos", torch.float32, 2)
     _need(sin, "sin", torch.float32, 2)
-    if positions.shape[0] != T or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
+    lmax, half = cos.shape
+    if positions.shape[0] != T or sin.shape != cos.shape or not cos.is_contiguous() or not sin.is_contiguous():
         raise ValueError("positions must be [T], cos and sin contiguous [lmax, rot / 2]")
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None:
             _need(w, name, torch.float32, 1)
             if w.shape[0] != HD:
                 raise ValueError("%s must be [%d]" % (name, HD))
-    q = torch.empty((T, NH, HD), dtype=qkv.dtype, device=qkv.device) if out is None else out
-    if q.dtype != qkv.dtype or tuple(q.shape) != (T, NH, HD) or not q.is_contiguous():
+    if out is None:
+        out = qkv.new_empty((T, NH, HD))
+    elif out.dtype != qkv.dtype or tuple(out.shape) != (T, NH, HD) or not out.is_contiguous():
         raise ValueError("out must be a contiguous %s tensor %s" % (qkv.dtype, (T, NH, HD)))
     k = None
     if cache is None:
-        k = torch.empty((T, NKV, HD), dtype=qkv.dtype, device=qkv.device)
-        where = (None, 0, 0, 0, None)
+        k = qkv.new_empty((T, NKV, HD))
+        where = (k.data_ptr(), None, 0, 0, 0, None)
     else:
         _need(slots, "slots", torch.int64, 1)
-        if (cache.NKV, cache.HD) != (NKV, HD) or slots.shape[0] != T:
+        if cache.NKV != NKV or cache.HD != HD or slots.shape[0] != T:
             raise ValueError("the cache holds %d heads of %d, and slots must be [T]" % (cache.NKV, cache.HD))
-        where = (cache.data.data_ptr(), cache.num_pages, cache.page, cache.group, slots.data_ptr())
-    _ffi.call("ql_qk_norm_rope", qkv.data_ptr(), _ffi.dtype_code(qkv.dtype), max(qkv.stride(0), qkv.shape[1]), T, NH, NKV,
-              HD, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
-              _ffi.ptr(q_weight), _ffi.ptr(k_weight), float(eps), q.data_ptr(), _ffi.ptr(k), *where,
-              _ffi.stream_ptr(stream, qkv.device))
-    return q, k
+        where = (None, cache.data.data_ptr(), cache.num_pages, cache.page, cache.group, slots.data_ptr())
+    _ffi.call("ql_qk_norm_rope", qkv.data_ptr(), _ffi.dtype_code(qkv.dtype), qkv.stride(0) if T > 1 else width, T, NH, NKV,
+              HD, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), lmax, 2 * half, _ffi.ptr(q_weight),
+              _ffi.ptr(k_weight), eps, out.data_ptr(), *where, _ffi.stream_ptr(stream, qkv.device))
+    return out, k
 
 
 def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=0, out=None, workspace=None,
@@ -171,16 +174,20 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
     (0: all). workspace: uint8 of ql_kv4_attention_workspace bytes, zeroed once and not shared by calls that
     overlap (None: one for each stream). Rows that see nothing, and rows past cu_q[B], are zero. Returns
     [T, NH, HD] in q's dtype."""
-    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
-        raise ValueError("q must be [T, NH, HD] with contiguous heads, got %s" % (tuple(q.shape),))
     _need(q, "q", q.dtype, 3)
     T, NH, HD = q.shape
+    ldq = NH * HD
+    dense = q.is_contiguous()
+    if not dense:
+        if q.stride(2) != 1 or q.stride(1) != HD:
+            raise ValueError("q must be [T, NH, HD] with contiguous heads, got %s, strides %s" % (tuple(q.shape), q.stride()))
+        ldq = q.stride(0)
     _need(block_table, "block_table", torch.int32, 2)
     _need(seq_lens, "seq_lens", torch.int32, 1)
-    B = seq_lens.shape[0]
-    if HD != cache.HD or NH % cache.NKV or block_table.shape[0] != B:
+    B, width = block_table.shape
+    if HD != cache.HD or NH % cache.NKV or seq_lens.shape[0] != B:
         raise ValueError("q has %d heads of %d, the cache %d of %d; block_table has %d rows for %d requests"
-                         % (NH, HD, cache.NKV, cache.HD, block_table.shape[0], B))
+                         % (NH, HD, cache.NKV, cache.HD, B, seq_lens.shape[0]))
     if cu_q is None:
         if T < B:
             raise ValueError("%d queries for %d requests" % (T, B))
@@ -188,17 +195,15 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
         _need(cu_q, "cu_q", torch.int32, 1)
         if cu_q.shape[0] != B + 1:
             raise ValueError("cu_q must be [%d]" % (B + 1))
-    ldq = q.stride(0) if T > 1 else NH * HD
     if q.data_ptr() % 16 or ldq * q.element_size() % 16:      # the kernel reads 16 bytes at a time
-        q, ldq = torch.empty((T, NH, HD), dtype=q.dtype, device=q.device).copy_(q), NH * HD
+        q, ldq, dense = torch.empty((T, NH, HD), dtype=q.dtype, device=q.device).copy_(q), NH * HD, True
     if out is None:
-        out = torch.empty((T, NH, HD), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if dense else q.new_empty((T, NH, HD))
     elif out.dtype != q.dtype or tuple(out.shape) != (T, NH, HD) or not out.is_contiguous():
         raise ValueError("out must be a contiguous %s tensor %s" % (q.dtype, (T, NH, HD)))
     ws = _attention_workspace(cache, NH, stream) if workspace is None else workspace
-    _ffi.call("ql_kv4_attention", q.data_ptr(), _ffi.dtype_code(q.dtype), ldq, T, NH, cache.NKV, HD,
-              cache.data.data_ptr(), cache.num_pages, cache.page, cache.group, block_table.data_ptr(),
-              max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], seq_lens.data_ptr(), _ffi.ptr(cu_q),
-              B, float(scale) if scale is not None else 1.0 / math.sqrt(HD), int(window), out.data_ptr(), ws.data_ptr(),
-              ws.numel(), _ffi.stream_ptr(stream, q.device))
+    _ffi.call("ql_kv4_attention", q.data_ptr(), _ffi.dtype_code(q.dtype), ldq, T, NH, cache.NKV, HD, cache.data.data_ptr(),
+              cache.num_pages, cache.page, cache.group, block_table.data_ptr(), block_table.stride(0) if B > 1 else width,
+              width, seq_lens.data_ptr(), _ffi.ptr(cu_q), B, HD ** -0.5 if scale is None else scale, window,
+              out.data_ptr(), ws.data_ptr(), ws.numel(), _ffi.stream_ptr(stream, q.device))
     return out
