@@ -41,7 +41,7 @@ constexpr int kPromptRows = 64;
 template <int HD>
 struct Shape {
   static constexpr int kWarps = HD == 64 ? 16 : HD == 128 ? 12 : 8;
-  static constexpr int kStages = HD == 256 ? 3 : 4;
+  static constexpr int kStages = 4;               // two pairs of blocks
   static constexpr int kThreads = kWarps * 32;
 };
 
@@ -176,29 +176,30 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, const Request& r
 constexpr float kLazy = 6.f;
 constexpr float kPShift = 9.f;   // p' = 2^9 p, up to 2^15: 11 bits of probabilities down to 2^-23
 
-// One block of 16 positions in shared memory. MASKED: some of its positions are not seen by some row.
-// lo / hi: visible positions of this lane's rows, relative to the block; any_lo / any_hi: of any row.
-// A masked position has p = 0, and where no row sees it its scales are dropped too, since memory that
-// was never written may hold codes for nan.
+// Two blocks of 16 positions in shared memory: what there is once for a step of the loop (waits, the maximum's
+// shuffles and vote) is once for 32 positions. MASKED: some of them are not seen by some row. lo / hi: visible
+// positions of this lane's rows, relative to the first block; any_lo / any_hi: of any row. A masked position
+// has p = 0, and where no row sees it its scales are dropped too, since memory that was never written may
+// hold codes for nan.
 template <int HD, int G, int PL, bool MASKED>
-__device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* blk, const uint4* qf,
-                                             const float (&coef)[3 - PL], const int (&lo)[3 - PL],
-                                             const int (&hi)[3 - PL], int any_lo, int any_hi) {
+__device__ __forceinline__ void attend_blocks(State<HD, PL>& st, const uint8_t* const (&blk)[2], const uint4* qf,
+                                              const float (&coef)[3 - PL], const int (&lo)[3 - PL],
+                                              const int (&hi)[3 - PL], int any_lo, int any_hi) {
   constexpr int R = 3 - PL;                 // rows of a lane
   constexpr int KW = HD / 32, VW = HD / 64; // words of a lane: keys of one position, values of one
-  constexpr int NG = HD / G;
+  constexpr int NG = HD / G, TWO = HD == 256 && G == 32 ? 2 : 1;   // groups that a lane's key elements are in
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint8_t* ks = blk + code_bytes(HD);
-  const uint8_t* vc = ks + scale_bytes(HD, G);
-  const uint8_t* vs = vc + code_bytes(HD);
-  float c[2][4] = {};                       // S of positions t, t + 4 | t + 8, t + 12
-  {
+  float z[R][8];                            // S of positions 16 b + t + 4 k, at 4 b + k
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const uint8_t* ks = blk[b] + code_bytes(HD);
+    float c[2][4] = {};                     // of positions t, t + 4 | t + 8, t + 12
     uint32_t w[2][KW];
-    __half2 sm[2][HD == 256 && G == 32 ? 2 : 1];   // a lane's elements are in one group, or two
+    __half2 sm[2][TWO];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = 8 * j + (g >> 1) + 4 * (g & 1);
-      const uint8_t* kp = blk + row * (HD / 2) + t * (HD / 8);
+      const uint8_t* kp = blk[b] + row * (HD / 2) + t * (HD / 8);
       if constexpr (KW >= 4) {
 #pragma unroll
         for (int i = 0; i < KW; i += 4) {
@@ -210,15 +211,14 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
         w[j][0] = u.x; w[j][1] = u.y;
       }
 #pragma unroll
-      for (int i = 0; i < (HD == 256 && G == 32 ? 2 : 1); ++i)
-        sm[j][i] = reinterpret_cast<const __half2*>(ks)[row * NG + (t * (HD / 4) + 32 * i) / G];
+      for (int i = 0; i < TWO; ++i) sm[j][i] = reinterpret_cast<const __half2*>(ks)[row * NG + (t * (HD / 4) + 32 * i) / G];
     }
 #pragma unroll
     for (int i = 0; i < KW; ++i) {
       const uint4 a0 = qf[(2 * i) * 32 + lane], a1 = qf[(2 * i + 1) * 32 + lane];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const __half2 u = sm[j][HD == 256 && G == 32 ? i / 4 : 0], s2 = __low2half2(u), m2 = __high2half2(u);
+        const __half2 u = sm[j][TWO == 2 ? i / 4 : 0], s2 = __low2half2(u), m2 = __high2half2(u);
         __half2 n[4];
         codes_h2(w[j][i], n);
 #pragma unroll
@@ -227,24 +227,23 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
         mma_16816_f16(c[j], a1.x, a1.y, a1.z, a1.w, h2_as_u32(n[2]), h2_as_u32(n[3]));
       }
     }
-  }
-  float z[R][4];                            // of positions t + 4 k
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (PL == 2) {
-        z[0][2 * j + k] = c[j][k] + c[j][k + 2];
-      } else {
-        z[0][2 * j + k] = c[j][k];
-        z[R - 1][2 * j + k] = c[j][k + 2];
+      for (int k = 0; k < 2; ++k) {
+        if (PL == 2) {
+          z[0][4 * b + 2 * j + k] = c[j][k] + c[j][k + 2];
+        } else {
+          z[0][4 * b + 2 * j + k] = c[j][k];
+          z[R - 1][4 * b + 2 * j + k] = c[j][k + 2];
+        }
       }
-    }
+  }
   if (MASKED) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 8; ++k)
         if (t + 4 * k < lo[r] || t + 4 * k >= hi[r]) z[r][k] = -INFINITY;
   }
   float mn[R];
@@ -252,6 +251,7 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float x = fmaxf(fmaxf(z[r][0], z[r][1]), fmaxf(z[r][2], z[r][3]));
+    x = fmaxf(x, fmaxf(fmaxf(z[r][4], z[r][5]), fmaxf(z[r][6], z[r][7])));
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
     mn[r] = MASKED && x == -INFINITY ? -INFINITY : x * coef[r];   // coef may be 0
@@ -274,12 +274,12 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
       st.o[i][3] *= f[R - 1];
     }
   }
-  uint32_t a[4];
+  uint32_t a[2][4];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float base = kPShift - (MASKED && st.m[r] == -INFINITY ? 0.f : st.m[r]);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 4; ++j) {
       float p[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -291,57 +291,62 @@ __device__ __forceinline__ void attend_block(State<HD, PL>& st, const uint8_t* b
       if (PL == 2) {
         __half2 h, l;
         split_h2(p[0], p[1], h, l);
-        a[2 * j] = h2_as_u32(h);
-        a[2 * j + 1] = h2_as_u32(l);
+        a[j >> 1][2 * (j & 1)] = h2_as_u32(h);
+        a[j >> 1][2 * (j & 1) + 1] = h2_as_u32(l);
       } else {
-        a[2 * j + r] = h2_as_u32(__floats2half2_rn(p[0], p[1]));
+        a[j >> 1][2 * (j & 1) + r] = h2_as_u32(__floats2half2_rn(p[0], p[1]));
       }
     }
   }
   // values: words of positions t, t + 4 | t + 8, t + 12, elements g HD / 8 ...
-  uint32_t w[4][VW];
-  __half2 s2[2], m2[2], sm[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint8_t* p = vc + (t + 4 * k) * (HD / 2) + g * (HD / 16);
-    if constexpr (VW == 4) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
-    } else if constexpr (VW == 2) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      w[k][0] = u.x; w[k][1] = u.y;
-    } else {
-      w[k][0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-    sm[k] = reinterpret_cast<const __half2*>(vs)[(t + 4 * k) * NG + g * (HD / 8) / G];
-  }
-  if (MASKED) {
+  for (int b = 0; b < 2; ++b) {
+    const uint8_t* vc = blk[b] + code_bytes(HD) + scale_bytes(HD, G);
+    const uint8_t* vs = vc + code_bytes(HD);
+    uint32_t w[4][VW];
+    __half2 s2[2], m2[2], sm[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (t + 4 * k < any_lo || t + 4 * k >= any_hi) sm[k] = h2_const(0u);
-  }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    s2[k] = __lows2half2(sm[2 * k], sm[2 * k + 1]);
-    m2[k] = __highs2half2(sm[2 * k], sm[2 * k + 1]);
-  }
-#pragma unroll
-  for (int i = 0; i < VW; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t sel = h ? 0x7632u : 0x5410u;
-      __half2 b0[4], b1[4];
-      // nibbles 0..3 of the half words of two positions: codes_h2 reads the interleaved word as
-      // (nibble j of one, nibble j of the other)
-      codes_h2(__byte_perm(w[0][i], w[1][i], sel), b0);
-      codes_h2(__byte_perm(w[2][i], w[3][i], sel), b1);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        b0[k] = __hfma2(b0[k], s2[0], m2[0]);
-        b1[k] = __hfma2(b1[k], s2[1], m2[1]);
-        mma_16816_f16(st.o[8 * i + 4 * h + k], a[0], a[1], a[2], a[3], h2_as_u32(b0[k]), h2_as_u32(b1[k]));
+    for (int k = 0; k < 4; ++k) {
+      const uint8_t* p = vc + (t + 4 * k) * (HD / 2) + g * (HD / 16);
+      if constexpr (VW == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
+      } else if constexpr (VW == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[k][0] = u.x; w[k][1] = u.y;
+      } else {
+        w[k][0] = *reinterpret_cast<const uint32_t*>(p);
       }
+      sm[k] = reinterpret_cast<const __half2*>(vs)[(t + 4 * k) * NG + g * (HD / 8) / G];
     }
+    if (MASKED) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (16 * b + t + 4 * k < any_lo || 16 * b + t + 4 * k >= any_hi) sm[k] = h2_const(0u);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      s2[k] = __lows2half2(sm[2 * k], sm[2 * k + 1]);
+      m2[k] = __highs2half2(sm[2 * k], sm[2 * k + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < VW; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t sel = h ? 0x7632u : 0x5410u;
+        __half2 b0[4], b1[4];
+        // nibbles 0..3 of the half words of two positions: codes_h2 reads the interleaved word as
+        // (nibble j of one, nibble j of the other)
+        codes_h2(__byte_perm(w[0][i], w[1][i], sel), b0);
+        codes_h2(__byte_perm(w[2][i], w[3][i], sel), b1);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          b0[k] = __hfma2(b0[k], s2[0], m2[0]);
+          b1[k] = __hfma2(b1[k], s2[1], m2[1]);
+          mma_16816_f16(st.o[8 * i + 4 * h + k], a[b][0], a[b][1], a[b][2], a[b][3], h2_as_u32(b0[k]), h2_as_u32(b1[k]));
+        }
+      }
+  }
 }
 
 template <int HD, int PL>
@@ -652,12 +657,15 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
       for (int j = 0; j < 4; ++j) st.o[i][j] = 0.f;
     uint32_t next = kNoBlock, missing = 0;
     __syncwarp();
-    for (int i = 0; i < n; ++i) {
+    for (int i = 0; i < n; i += 2) {
       if ((i & 31) == 0) {                        // lane j looks up block j of the 32 after these
         missing = __ballot_sync(0xffffffffu, src == kNoBlock);
         next = source(a, c.b, c.kvh, blk0, i + 32 + lane, n);
       }
-      if (!ptx::mbar_wait(bar + 8 * s, phase, &abort_flag)) {
+      const bool both = i + 1 < n;
+      const int s1 = s + 1 == ST ? 0 : s + 1;
+      if (!ptx::mbar_wait(bar + 8 * s, phase, &abort_flag) ||
+          (both && !ptx::mbar_wait(bar + 8 * s1, phase ^ (s1 == 0), &abort_flag))) {
         // gave up: nan for this tile, and no copy left in flight
         bad = true;
         for (int j = i; j < min(i + ST, n); ++j) {
@@ -666,26 +674,29 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
         }
         break;
       }
-      if ((missing >> (i & 31)) & 1) {
-        bad = true;                               // a page that is not one of the cache's: nan
-      } else if (i >= first_seen && i < first_masked) {
+      // a page that is not one of the cache's: nan
+      bad = bad || ((missing >> (i & 31)) & 1) || (both && ((missing >> (i & 31)) & 2));
+      const uint8_t* const blk[2] = {ring + s * BB, ring + s1 * BB};
+      if (i >= first_seen && i + 1 < first_masked && both) {
         const int all[R] = {};
-        attend_block<HD, G, PL, false>(st, ring + s * BB, qf, coef, all, all, 0, kBlock);
+        attend_blocks<HD, G, PL, false>(st, blk, qf, coef, all, all, 0, 2 * kBlock);
       } else {
-        const int p0 = (blk0 + i) * kBlock;
+        // (of a second block past the last one nothing is seen)
+        const int p0 = (blk0 + i) * kBlock, end = both ? 2 * kBlock : kBlock;
         int lo[R], hi[R];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
           lo[j] = (a.window ? max(pos[j] - a.window + 1, 0) : 0) - p0;
-          hi[j] = pos[j] + 1 - p0;
+          hi[j] = min(pos[j] + 1 - p0, end);
         }
-        attend_block<HD, G, PL, true>(st, ring + s * BB, qf, coef, lo, hi, c.lo_all - p0, c.hi_all - p0);
+        attend_blocks<HD, G, PL, true>(st, blk, qf, coef, lo, hi, c.lo_all - p0, min(c.hi_all - p0, end));
       }
       __syncwarp();
-      const int ahead = i + ST;                  // the stage is free: block i + ST goes there
-      if (ahead < n && (ahead & 31) == lane) issue<BB>(a, (ahead ^ i) & 32 ? next : src, s, ring_s, bar);
-      if ((i & 31) == 31) src = next;
-      if (++s == ST) s = 0, phase ^= 1;
+      // the stages are free: blocks i + ST and i + ST + 1 go there
+      const int ahead = i + ST + (lane & 1);
+      if (ahead < n && (ahead & 31) == lane) issue<BB>(a, (ahead ^ i) & 32 ? next : src, lane & 1 ? s1 : s, ring_s, bar);
+      if ((i & 31) == 30) src = next;
+      if ((s += both ? 2 : 1) >= ST) s -= ST, phase ^= 1;
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
