@@ -368,56 +368,6 @@ __device__ __forceinline__ void store_part(const State<HD, PL>& st, float* part)
     }
 }
 
-template <int HD, int PL>
-__device__ __forceinline__ void copy_part(float* to, const float* from) {
-  for (int i = threadIdx.x & 31; i < Part<HD, PL>::kFloats / 4; i += 32)
-    reinterpret_cast<float4*>(to)[i] = reinterpret_cast<const float4*>(from)[i];
-}
-
-// st joined with n parts in shared memory, in their order.
-template <int HD, int PL>
-__device__ __forceinline__ void join_parts(State<HD, PL>& st, const float* part, int n) {
-  constexpr int SIZE = Part<HD, PL>::kFloats;
-  const int lane = threadIdx.x & 31;
-  float top[3 - PL], f[3 - PL];
-#pragma unroll
-  for (int r = 0; r < 3 - PL; ++r) {
-    const float* ml = part + Part<HD, PL>::kStats + (lane >> 2) + 8 * r;
-    top[r] = st.m[r];
-    for (int p = 0; p < n; ++p) top[r] = fmaxf(top[r], ml[p * SIZE]);
-    const float base = top[r] == -INFINITY ? 0.f : top[r];
-    f[r] = ex2(st.m[r] - base);
-    st.m[r] = top[r];
-    st.l[r] *= f[r];
-    top[r] = base;
-  }
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i) {
-    st.o[i][0] *= f[0];
-    st.o[i][1] *= f[0];
-    st.o[i][2] *= f[2 - PL];
-    st.o[i][3] *= f[2 - PL];
-  }
-  for (int p = 0; p < n; ++p, part += SIZE) {
-#pragma unroll
-    for (int r = 0; r < 3 - PL; ++r) {
-      const float* ml = part + Part<HD, PL>::kStats + (lane >> 2) + 8 * r;
-      f[r] = ex2(ml[0] - top[r]);
-      st.l[r] = fmaf(f[r], ml[16], st.l[r]);
-    }
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
-      const auto v = reinterpret_cast<const typename Vec<4 / PL>::T*>(part)[i * 32 + lane];
-      st.o[i][0] = fmaf(f[0], v.x, st.o[i][0]);
-      st.o[i][1] = fmaf(f[0], v.y, st.o[i][1]);
-      if constexpr (PL == 1) {
-        st.o[i][2] = fmaf(f[1], v.z, st.o[i][2]);
-        st.o[i][3] = fmaf(f[1], v.w, st.o[i][3]);
-      }
-    }
-  }
-}
-
 template <int DT>
 __device__ __forceinline__ void store2(void* out, long i, float x, float y) {
   if (DT == QL_F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(out) + i) = make_float2(x, y);
@@ -512,16 +462,17 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
   for (long i = used + (long)blockIdx.x * NT + tid; i < all; i += (long)gridDim.x * NT)
     store_from_float(a.out, DT, i, 0.f);
 
-  // the line of units: where this warp's piece begins. Up to 32 requests each warp finds it alone;
+  // the line of units: where this warp's piece begins. Up to 256 requests each warp finds it alone;
   // for more, every thread sums some requests and the block adds up.
   const long long w0 = (long long)blockIdx.x * NW;
   long long W = 0, us = 0;                     // units in all, and before request b
   int b = 0;
   Request r = {};
   Split split;
-  if (a.B <= 32) {
-    if (lane < a.B) r = load_request<ROWS>(a, lane);
-    const long long mine = lane < a.B ? units_of(r, a.NKV) : 0;
+  if (a.B <= 256) {
+    const int each = (a.B + 31) / 32, b0 = min(lane * each, a.B), b1 = min(b0 + each, a.B);
+    long long mine = 0;
+    for (int i = b0; i < b1; ++i) mine += units_of(load_request<ROWS>(a, i), a.NKV);
     long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -531,14 +482,17 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
     W = __shfl_sync(0xffffffffu, incl, 31);
     split = Split(W, gridDim.x * NW);
     if (w0 >= split.warps) return;
-    b = min(__popc(__ballot_sync(0xffffffffu, incl <= split.start(w0 + warp))), 31);
-    us = __shfl_sync(0xffffffffu, incl - mine, b);
-    r.q0 = __shfl_sync(0xffffffffu, r.q0, b);
-    r.ql = __shfl_sync(0xffffffffu, r.ql, b);
-    r.seq = __shfl_sync(0xffffffffu, r.seq, b);
-    r.tiles = __shfl_sync(0xffffffffu, r.tiles, b);
-    r.blo = __shfl_sync(0xffffffffu, r.blo, b);
-    r.nblk = __shfl_sync(0xffffffffu, r.nblk, b);
+    if (w0 + warp < split.warps) {
+      const long long u = split.start(w0 + warp);
+      const int owner = __popc(__ballot_sync(0xffffffffu, incl <= u));   // the lane whose requests it is among
+      us = __shfl_sync(0xffffffffu, incl - mine, owner);
+      b = min(owner * each, a.B - 1);
+      for (;; ++b) {
+        r = load_request<ROWS>(a, b);
+        if (u < us + units_of(r, a.NKV)) break;
+        us += units_of(r, a.NKV);
+      }
+    }
   } else {
     const int each = (a.B + NT - 1) / NT, b0 = min(tid * each, a.B), b1 = min(b0 + each, a.B);
     long long mine = 0;
@@ -719,117 +673,156 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
   }
   __syncthreads();
 
-  // join the parts of this CTA's warps: a tile's parts are in consecutive warps, and the warp where it
-  // begins (warp 0 for one that began in another CTA) takes the others in their order. The parts move
-  // to shared memory, where the rings and queries are done with.
-  constexpr int SIZE = Part<HD, PL>::kFloats;
+  // Join the parts of this CTA's warps: a tile's parts are in consecutive warps, and the warp where it begins
+  // (warp 0 for one that began in another CTA) adds them up in their order. A warp's last part goes to shared
+  // memory, where the rings and queries are done with; an earlier one is in the workspace. Loops over
+  // four floats at a time, not straight code over the state: it runs once, and its instructions have to be fetched.
+  constexpr int SIZE = Part<HD, PL>::kFloats, STATS = Part<HD, PL>::kStats;
   float* shared_parts = reinterpret_cast<float*>(smem);
   static_assert(NW * SIZE * 4 <= L::kBar, "the parts of a CTA's warps fit where its rings were");
-  const bool last_is_head = c.item0 < c.u0 && c.head;
-  if (c.head && warp > 0) {
-    if (last_is_head) {
-      store_part<HD, PL>(st, shared_parts + warp * SIZE);
-    } else {
-      copy_part<HD, PL>(shared_parts + warp * SIZE, parts + (2 + warp) * SIZE);
-    }
-  }
+  if (c.u0 < c.u1 && (c.item0 < c.u0 || c.item1 > c.u1)) store_part<HD, PL>(st, shared_parts + warp * SIZE);
   __syncthreads();
-  // parts that follow this warp's, and whether the tile ends with them
-  const auto following = [&](bool& open) {
-    int n = 0;
+  const auto head_part = [&](int w) {
+    return pieces[w].item0 < pieces[w].u0 ? shared_parts + w * SIZE : parts + (2 + w) * SIZE;
+  };
+  // four floats i of a part are two neighbouring lanes of a fragment, or one lane's two rows: to the output, lane
+  // (g, t) of tile k has elements 2t HD / 8 + k and HD / 8 past it
+  const auto put = [&](const Cross& x, int i, float4 v, float f0, float f1) {
+    const int ln = i * PL & 31, gg = ln >> 2, e = 2 * (ln & 3) * (HD / 8) + (i * PL >> 5);
+    const float o[4] = {v.x * f0, v.y * f0, v.z * (PL == 2 ? f0 : f1), v.w * (PL == 2 ? f0 : f1)};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = PL == 2 ? gg : gg + 8 * h;
+      if (row >= x.nrows) continue;
+      const long at = out_row(a, x.q0, x.kvh, x.r0 + row, grp) * HD + (PL == 2 ? e + 2 * h * (HD / 8) : e);
+      store_from_float(a.out, DT, at, o[2 * h]);
+      store_from_float(a.out, DT, at + HD / 8, o[2 * h + 1]);
+    }
+  };
+#pragma unroll 1
+  for (int run = 0; run < 2; ++run) {
+    // 0: the tile that began in an earlier CTA, 1: one that begins in this warp and goes on
+    if (!(run == 0 ? warp == 0 && c.head : c.item1 > c.u1 && c.item0 >= c.u0)) continue;
+    bool open = run ? true : c.whole;            // goes on past the parts so far
+    int n = 1;
     for (int w = warp + 1; open && w < NW && pieces[w].head; ++w) {
       ++n;
       open = pieces[w].whole;
     }
-    return n;
-  };
-  if (warp == 0 && c.head) {
-    if (last_is_head) {
-      bool open = c.whole;
-      const int n = following(open);
-      join_parts<HD, PL>(st, shared_parts + SIZE, n);
-      store_part<HD, PL>(st, parts);
-    } else {                                     // its state went on to another tile: the part is as it was
-      copy_part<HD, PL>(parts, parts + 2 * SIZE);
+    constexpr int CH = HD / 8 / PL;              // fours of a lane: all of one row, or of two
+    const int row = (PL == 2 ? 2 * lane & 31 : lane) >> 2;
+    float m[R], l[R] = {}, base[R];
+    float4 acc[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto part = [&](int p) -> const float* {
+      return p == 0 && run ? shared_parts + warp * SIZE : head_part(warp + p);
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = -INFINITY;
+      for (int p = 0; p < n; ++p) m[r] = fmaxf(m[r], part(p)[STATS + row + 8 * r]);
+      base[r] = m[r] == -INFINITY ? 0.f : m[r];
     }
-  }
-  if (c.item1 > c.u1 && c.item0 >= c.u0) {       // a tile that begins here and goes on
-    bool open = true;
-    const int n = following(open);
-    join_parts<HD, PL>(st, shared_parts + (warp + 1) * SIZE, n);
-    if (!open) {
-      write_tile<DT, HD, PL>(a, st, c.r.q0, c.kvh, c.r0, c.nrows, grp);
-    } else {
-      if (lane == 0)
-        cross[1] = {1, c.r.q0, c.kvh, c.r0, c.nrows, (int)blockIdx.x, sh_split.warp_of(c.item1 - 1) / NW, 0};
-      store_part<HD, PL>(st, parts + SIZE);
+#pragma unroll 1
+    for (int p = 0; p < n; ++p) {
+      const float* from = part(p);
+      float f[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        f[r] = ex2(from[STATS + row + 8 * r] - base[r]);
+        l[r] = fmaf(f[r], from[STATS + 16 + row + 8 * r], l[r]);
+      }
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const float4 v = reinterpret_cast<const float4*>(from)[i * 32 + lane];
+        acc[i].x = fmaf(f[0], v.x, acc[i].x);
+        acc[i].y = fmaf(f[0], v.y, acc[i].y);
+        acc[i].z = fmaf(f[R - 1], v.z, acc[i].z);
+        acc[i].w = fmaf(f[R - 1], v.w, acc[i].w);
+      }
     }
+    if (run && !open) {
+      const Cross x = {1, c.r.q0, c.kvh, c.r0, c.nrows, 0, 0, 0};
+      const float f0 = l[0] == 0.f ? 0.f : 1.f / l[0], f1 = l[R - 1] == 0.f ? 0.f : 1.f / l[R - 1];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) put(x, i * 32 + lane, acc[i], f0, f1);
+      continue;
+    }
+    float* to = parts + run * SIZE;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) reinterpret_cast<float4*>(to)[i * 32 + lane] = acc[i];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      to[STATS + row + 8 * r] = m[r];
+      to[STATS + 16 + row + 8 * r] = l[r];
+    }
+    if (run && lane == 0)
+      cross[1] = {1, c.r.q0, c.kvh, c.r0, c.nrows, (int)blockIdx.x, sh_split.warp_of(c.item1 - 1) / NW, 0};
   }
   if (tid == 0 && abort_flag) atomicExch(&g_kv4_status, 1);
-  __threadfence();
   __syncthreads();
   if (tid < 2 && cross[tid].valid) {
-    // of the CTAs that share the tile, the last to arrive joins their parts
+    // of the CTAs that share the tile, the last to arrive joins their parts (the fence covers what the
+    // barrier has shown this thread of the other threads' stores)
     const Cross x = cross[tid];
+    __threadfence();
     const bool done = atomicAdd(&a.counters[x.first], 1u) == (unsigned)(x.last - x.first);
     if (done) a.counters[x.first] = 0u;
+    __threadfence();
     cross[tid].finish = done;
   }
   __syncthreads();
-  float* weight = reinterpret_cast<float*>(smem);   // [parts][16], in the ring, which is idle now
+  float* stats = reinterpret_cast<float*>(smem);    // [parts][m of 16 rows, l of 16 rows]
+#pragma unroll 1
   for (int k = 0; k < 2; ++k) {
     const Cross x = cross[k];
     if (!x.valid || !x.finish) continue;
-    __threadfence();
     const int n = x.last - x.first + 1;
-    const auto part_of = [&](int p) {
+    const auto part = [&](int p) {
       return a.parts + ((long)(x.first + p) * (2 + NW) + (p == 0 ? 1 : 0)) * SIZE;
     };
-    float* top = weight + n * 16;                // the parts' m, then l
-    for (int i = tid; i < n * 16; i += NT) {
-      const float* ml = part_of(i >> 4) + Part<HD, PL>::kStats + (i & 15);
-      top[i] = __ldcg(ml);
-      top[n * 16 + i] = __ldcg(ml + 16);
-    }
-    __syncthreads();
-    for (int row = warp; row < ROWS; row += NW) {
-      float m = -INFINITY, l = 0.f;
-      for (int p = lane; p < n; p += 32) m = fmaxf(m, top[p * 16 + row]);
+    constexpr int NQ = HD / 4 * 16 / PL, AHEAD = 8;
+    float4 v[AHEAD];                             // the first parts, under way with the stats
+    if (tid < NQ)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float base = m == -INFINITY ? 0.f : m;
-      for (int p = lane; p < n; p += 32) l = fmaf(ex2(top[p * 16 + row] - base), top[(n + p) * 16 + row], l);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      for (int p = lane; p < n; p += 32) weight[p * 16 + row] = ex2(top[p * 16 + row] - base) * inv;
-    }
+      for (int p = 0; p < AHEAD; ++p)
+        if (p < n) v[p] = __ldcg(reinterpret_cast<const float4*>(part(p)) + tid);
+    for (int i = tid; i < n * 32; i += NT) stats[i] = __ldcg(part(i >> 5) + STATS + (i & 31));
     __syncthreads();
-    // four floats a thread: two neighbouring lanes of a fragment, or one lane's two rows
-    for (int i = tid; i < HD / 8 * 32 / PL; i += NT) {
-      const int ln = i * PL & 31, gg = ln >> 2, tile = i * PL >> 5;
+#pragma unroll 1
+    for (int i = tid; i < NQ; i += NT) {
+      const int row = (i * PL & 31) >> 2;
+      float base[R], l[R] = {};
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float m = -INFINITY;
+        for (int p = 0; p < n; ++p) m = fmaxf(m, stats[p * 32 + row + 8 * r]);
+        base[r] = m == -INFINITY ? 0.f : m;
+      }
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 16
-      for (int p = 0; p < n; ++p) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(p)) + i);
-        const float f0 = weight[p * 16 + gg], f1 = PL == 2 ? f0 : weight[p * 16 + 8 + gg];
-        acc.x = fmaf(f0, v.x, acc.x);
-        acc.y = fmaf(f0, v.y, acc.y);
-        acc.z = fmaf(f1, v.z, acc.z);
-        acc.w = fmaf(f1, v.w, acc.w);
-      }
-      // lane (g, t) of tile i: elements 2t HD / 8 + i and HD / 8 past it
-      const int e = 2 * (ln & 3) * (HD / 8) + tile;
-      const float out[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll 1
+      for (int p0 = 0; p0 < n; p0 += AHEAD) {
+        if (i != tid || p0)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = PL == 2 ? gg : gg + 8 * h, at = PL == 2 ? e + 2 * h * (HD / 8) : e;
-        if (row < x.nrows) {
-          const long o = out_row(a, x.q0, x.kvh, x.r0 + row, grp) * HD + at;
-          store_from_float(a.out, DT, o, out[2 * h]);
-          store_from_float(a.out, DT, o + HD / 8, out[2 * h + 1]);
-        }
+          for (int p = 0; p < AHEAD; ++p)
+            if (p0 + p < n) v[p] = __ldcg(reinterpret_cast<const float4*>(part(p0 + p)) + i);
+#pragma unroll
+        for (int p = 0; p < AHEAD; ++p)
+          if (p0 + p < n) {
+            float f[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              f[r] = ex2(stats[(p0 + p) * 32 + row + 8 * r] - base[r]);
+              l[r] = fmaf(f[r], stats[(p0 + p) * 32 + 16 + row + 8 * r], l[r]);
+            }
+            acc.x = fmaf(f[0], v[p].x, acc.x);
+            acc.y = fmaf(f[0], v[p].y, acc.y);
+            acc.z = fmaf(f[R - 1], v[p].z, acc.z);
+            acc.w = fmaf(f[R - 1], v[p].w, acc.w);
+          }
       }
+      put(x, i, acc, l[0] == 0.f ? 0.f : 1.f / l[0], l[R - 1] == 0.f ? 0.f : 1.f / l[R - 1]);
     }
     __syncthreads();
   }
