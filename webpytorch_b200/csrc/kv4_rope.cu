@@ -142,19 +142,54 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
     reinterpret_cast<__half2*>(blk + code_bytes(HD))[r * (HD / a.group) + lane / gl] = __halves2half2(s, m);
 }
 
-// rint(d / s) for 0 <= d / s < 2^22 and s a half, as IEEE division rounds it. The product with 1 / s is off by a
-// rounding or two, which matters next to k + 1/2 only, and there the comparison is exact: (k + 1/2) s and
-// d - n s are fp32 numbers, and no d other than (k + 1/2) s itself has a quotient that rounds to k + 1/2 (a
-// neighbour of d is further off, relatively, than half a step of the quotient).
-__device__ __forceinline__ float round_quotient(float d, float s, float inv) {
-  constexpr float kMagic = 12582912.f;             // 1.5 * 2^23: the sum rounds to an integer, ties to even
-  float n = __fsub_rn(__fadd_rn(__fmul_rn(d, inv), kMagic), kMagic);
-  const float rest = fmaf(-n, s, d), half = 0.5f * s;
-  if (fabsf(rest) >= half) {
-    const bool odd = __float_as_int(__fadd_rn(n, kMagic)) & 1;
-    if (fabsf(rest) > half || odd) n += rest > 0.f ? 1.f : -1.f;
+// Pairs of IEEE fp32 operations in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// rint(d / s) for 0 <= d <= 15 s and s a half, as IEEE division rounds it, packed 4 bits each. The product with
+// 1 / s is off by a rounding or two, which matters next to k + 1/2 only, and there the comparison is exact:
+// (k + 1/2) s and d - n s are fp32 numbers, and no d other than (k + 1/2) s itself has a quotient that rounds to
+// k + 1/2 (a neighbour of d is further off, relatively, than half a step of the quotient). All elements are
+// looked at at once whether one is that near; an integer is the low bits of the sum with 1.5 * 2^23.
+template <int E>
+__device__ __forceinline__ uint32_t round_quotients(const float (&d)[E], float s, float inv) {
+  constexpr float kMagic = 12582912.f;
+  constexpr uint32_t kBits = 0x4B400000u;
+  const float half = 0.5f * s;
+  float t[E], near = 0.f;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    t[j] = __fadd_rn(__fmul_rn(d[j], inv), kMagic);             // ties to even
+    near = fmaxf(near, fabsf(fmaf(-__fsub_rn(t[j], kMagic), s, d[j])));
   }
-  return n;
+  if (near >= half) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float rest = fmaf(-__fsub_rn(t[j], kMagic), s, d[j]);
+      if (fabsf(rest) > half || (fabsf(rest) == half && (__float_as_uint(t[j]) & 1u))) t[j] += rest > 0.f ? 1.f : -1.f;
+    }
+  }
+  uint32_t code = 0u, offset = 0u;
+#pragma unroll
+  for (int j = E - 1; j >= 0; --j) {                            // (code << 4) + n, with the bits of 1.5 * 2^23 in it
+    code = code * 16u + __float_as_uint(t[j]);
+    offset = offset * 16u + kBits;
+  }
+  return code - offset;
 }
 
 // Rows of 16-byte aligned heads whose rotated halves are whole 16-byte pieces: a lane holds E consecutive
@@ -232,33 +267,29 @@ __device__ __forceinline__ void store_codes(const RopeArgs& a, const Token<DT, H
                                             const float (&x)[Lanes<DT, HD>::E]) {
   constexpr int E = Lanes<DT, HD>::E;
   const int gl = a.group / E;
-  float lo = x[0], hi = x[0], most = fabsf(x[0]);
-  bool ok = most <= 65504.f;
+  float lo = x[0], hi = x[0], zero = 0.f;
 #pragma unroll
-  for (int j = 1; j < E; ++j) {
+  for (int j = 0; j < E; ++j) {
     lo = fminf(lo, x[j]);
     hi = fmaxf(hi, x[j]);
-    if (DT != QL_F16) ok = ok && fabsf(x[j]) <= 65504.f;
-    else ok = ok && fabsf(x[j]) < INFINITY;
+    zero = fmaf(x[j], 0.f, zero);                    // nan where an element is not finite
   }
-  if (!ok) hi = INFINITY;
+  if (!(zero == 0.f)) hi = INFINITY;
   for (int o = 1; o < gl; o <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  ok = hi <= 65504.f;
+  const bool ok = hi <= 65504.f && lo >= -65504.f;
   __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)), m = __float2half_rn(lo);
   if (!ok) s = m = __ushort_as_half((unsigned short)0x7fff);
   const float sf = __half2float(s), mf = __half2float(m);
   const bool flat = !(sf > 0.f);                     // constant, or not finite: codes 0
   const float inv = flat ? 0.f : __frcp_rn(sf), step = flat ? 1.f : sf;
-  uint32_t code = 0;
+  float d[E];
+  // below zero by the minimum's rounding, above 15 steps by that and the scale's
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    // below zero by the minimum's rounding, above 15 by the scale's
-    const float d = flat ? 0.f : fminf(fmaxf(__fsub_rn(x[j], mf), 0.f), 15.f * step);
-    code |= (uint32_t)__float2int_rn(round_quotient(d, step, inv)) << (4 * j);
-  }
+  for (int j = 0; j < E; ++j) d[j] = fminf(fmaxf(__fsub_rn(x[j], mf), 0.f), flat ? 0.f : 15.f * step);
+  const uint32_t code = round_quotients<E>(d, step, inv);
   if (h < 0) return;
   uint8_t* to = k.blk + h * k.head_bytes + (is_v ? code_bytes(HD) + scale_bytes(HD, a.group) : 0);
   uint8_t* cp = to + k.r * (HD / 2) + l * (E / 2);
@@ -305,7 +336,11 @@ __device__ __forceinline__ void heads(const RopeArgs& a, const Token<DT, HD>& k,
         if (w) {
           float s[E];
 #pragma unroll
-          for (int j = 0; j < E; ++j) s[j] = __fmul_rn(x[j], x[j]);
+          for (int j = 0; j < E; j += 2) {
+            const float2 v = mul2(make_float2(x[j], x[j + 1]), make_float2(x[j], x[j + 1]));
+            s[j] = v.x;
+            s[j + 1] = v.y;
+          }
 #pragma unroll
           for (int n = E; n > 1; n /= 2)
 #pragma unroll
@@ -315,14 +350,20 @@ __device__ __forceinline__ void heads(const RopeArgs& a, const Token<DT, HD>& k,
           for (int o = 1; o < L::LPH; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
           const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
 #pragma unroll
-          for (int j = 0; j < E; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], inv), g[j]);
+          for (int j = 0; j < E; j += 2) {
+            const float2 v = mul2(mul2(make_float2(x[j], x[j + 1]), make_float2(inv, inv)), make_float2(g[j], g[j + 1]));
+            x[j] = v.x;
+            x[j + 1] = v.y;
+          }
         }
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
+        for (int j = 0; j < E; j += 2) {
           // x c - y s is x c + y (-s) to the bit
-          const float y = __shfl_sync(0xffffffffu, x[j], k.partner);
-          const float z = __fadd_rn(__fmul_rn(x[j], k.c[j]), __fmul_rn(y, k.s[j]));
-          x[j] = FULL || k.turns ? z : x[j];
+          const float2 y = make_float2(__shfl_sync(0xffffffffu, x[j], k.partner), __shfl_sync(0xffffffffu, x[j + 1], k.partner));
+          const float2 z = add2(mul2(make_float2(x[j], x[j + 1]), make_float2(k.c[j], k.c[j + 1])),
+                                mul2(y, make_float2(k.s[j], k.s[j + 1])));
+          x[j] = FULL || k.turns ? z.x : x[j];
+          x[j + 1] = FULL || k.turns ? z.y : x[j + 1];
         }
         if (!k.in)
 #pragma unroll
