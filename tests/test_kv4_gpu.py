@@ -321,6 +321,55 @@ def test_prompts(dtype, HD, NH, NKV, page, group, lens, ql, window):
     q, cu = bt.queries(ql, NH, dtype)
     bt.check(q, cu, attend(bt, q, cu, window=window), dtype, window)
 
+# calls with enough rows for the tensor-core kernel: long requests beside short, odd and empty ones
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("HD,NH,NKV,page,group,lens,ql", [
+    (128, 32, 4, 64, 64, [300, 77, 17, 0, 129], [200, 1, 9, 0, 3]), (128, 28, 4, 16, 128, [513, 640], [130, 101]),
+    (128, 40, 8, 32, 32, [1, 257, 128], [1, 193, 13]), (128, 8, 8, 16, 64, [900], [800]), (64, 64, 4, 32, 32, [257, 90, 260], [150, 1, 129]),
+    (64, 16, 16, 16, 64, [1000], [800]), (64, 14, 2, 64, 32, [1023, 64], [900, 1]), (256, 16, 2, 16, 64, [333, 20], [200, 20]),
+    (256, 16, 2, 32, 32, [70, 129, 5], [20, 129, 1]), (256, 40, 8, 16, 128, [400], [60]),
+])
+@pytest.mark.parametrize("window", [0, 1, 130])
+def test_many_rows(dtype, HD, NH, NKV, page, group, lens, ql, window):
+    bt = Batch(lens, NKV, HD, page, group, sum(lens) + window)
+    q, cu = bt.queries(ql, NH, dtype)
+    bt.check(q, cu, attend(bt, q, cu, window=window), dtype, window)
+
+
+@pytest.mark.parametrize("HD,NH,NKV", [(64, 64, 8), (128, 32, 8), (256, 16, 4)])
+def test_many_rows_that_see_nothing_bad_pages_and_streams(HD, NH, NKV):
+    """More query tokens than positions; a page that is not the cache's; a length past the table."""
+    bt = Batch([100, 250, 250, 40], NKV, HD, 16, 64, HD)
+    q, cu = bt.queries([200, 250, 250, 3], NH, "bf16")
+    good = attend(bt, q, cu)
+    bt.check(q, cu, good, "bf16")
+    assert (good[:100] == 0).all() and (good[100:] != 0).any()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    again = attend(bt, q, cu, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(good, again)
+    bt.table[1, 2] = -7
+    lens = dev(np.array([100, 250, 16 * bt.table.shape[1] + 1, 40], np.int32))
+    got = kv4.attention(q, bt.cache, bt.table, lens, dev(cu))
+    # the other requests: the cut of the work depends on all lengths, so not to the bit
+    bt.check(q, cu, torch.cat([got[:200], good[200:700], got[700:]]), "bf16")
+    # a row that sees the page, or any of the too long request, is nan
+    assert got[200 + 32:450].isnan().all() and got[450:700].isnan().all()
+
+
+def test_strided_queries_padding_scale_and_offsets_past_32_bits_for_many_rows():
+    first = (1 << 32) // (2304 * 4) + 5
+    bt = Batch([300, 33], 4, 128, 16, 64, 12, first_page=first)
+    q, cu = bt.queries([290, 4], 32, "f16")
+    wide = torch.full((300, 32 * 128 + 24), float("nan"), dtype=torch.float16, device=DEV)
+    wide[:294, :4096] = q.reshape(294, 4096)
+    out = torch.full((300, 32, 128), 7.0, dtype=torch.float16, device=DEV)
+    assert attend(bt, wide[:, :4096].unflatten(1, (32, 128)), cu, scale=-0.05, out=out) is out
+    bt.check(q, cu, out, "f16", scale=-0.05)
+    assert (out[294:] == 0).all()
+
+
 
 def test_strided_queries_scale_padding_and_out():
     bt = Batch([20, 33], 2, 64, 16, 32, 5)

@@ -828,6 +828,16 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
   }
 }
 
+// Whether requests of kPromptRows rows or more are the prompt kernel's. It takes 16 positions of 16 rows in a
+// fifth of the streaming kernel's time (0.16 against 0.8 ns at HD = 128), but walks the positions of 256 rows in
+// one CTA, 17 ns each, where the streaming kernel cuts them over all: at rows x heads / 256 x 0.8 ns a position
+// the two are level whatever the length. The host knows the tokens past one a request. Measured, both sides,
+// bf16, 32 heads over 4, 6000 positions: 128 query tokens 118 us (streaming 85), 256 119 (148), 2000 204 (1014);
+// 8 x 17 tokens over 3000 66 (60), 8 x 32 70 (87); 16 heads of 64, 3000 positions: 256 tokens 59 (35), 1000 60 (84).
+bool prompts_pay(int T, int B, int NH, int HD, int dtype) {
+  return dtype != QL_F32 && HD <= 128 && (long)(T - B) * NH * HD >= 3l << 18;
+}
+
 int sm_count() {
   int sms = 148, dev = 0;
   cudaGetDevice(&dev);
@@ -837,7 +847,7 @@ int sm_count() {
 
 template <int HD>
 constexpr size_t part_floats() {
-  return (size_t)(2 + Shape<HD>::kWarps) * (HD == 256 ? Part<HD, 2>::kFloats : Part<HD, 1>::kFloats);
+  return (size_t)(2 + Shape<HD>::kWarps) * Part<HD, 1>::kFloats;
 }
 size_t parts_bytes(int HD, int ctas) {
   return (HD == 64 ? part_floats<64>() : HD == 128 ? part_floats<128>() : part_floats<256>()) * ctas * sizeof(float);
@@ -861,8 +871,10 @@ int launch_one(const AttnArgs& a, int ctas, cudaStream_t st) {
 
 template <int DT, int HD, int G>
 int launch(const AttnArgs& a, int ctas, cudaStream_t st) {
-  // one plane where 16-bit inputs fill more than 8 rows: their outputs keep no more than the 11 bits
-  // of a single fp16 probability (HD = 256 has no registers for 16 rows)
+  // One plane where 16-bit inputs fill more than 8 rows of a tile: their outputs keep no more than the 11 bits of a
+  // single fp16 probability. The host knows the mean only. Measured, 64 requests of 4000 positions, bf16, HD = 128,
+  // one plane (two planes): 32 heads over 8, 1 token 103 us (99), 3 tokens 107 (183); over 4, 1 token 62 (58),
+  // 2 tokens 66 (100). HD = 256, 32 requests: 32 over 4, 1 token 63.6 (63.4), 2 tokens 80 (101).
   constexpr bool can = HD != 256 && DT != QL_F32;
   if (can && (long)a.T * (a.NH / a.NKV) > 8L * a.B) return launch_one<DT, HD, G, can ? 1 : 2>(a, ctas, st);
   return launch_one<DT, HD, G, 2>(a, ctas, st);
@@ -948,9 +960,7 @@ extern "C" int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int N
   a.B = B;
   a.scale = scale;
   a.window = window;
-  // at least half of a prompt tile's rows; the host knows only that no request has more than T - B + 1 tokens
-  // where each has one
-  a.prompt_rows = dtype != QL_F32 && HD <= 128 && (long)T * (NH / NKV) >= kPromptRows ? kPromptRows : 0;
+  a.prompt_rows = prompts_pay(T, B, NH, HD, dtype) ? kPromptRows : 0;
   a.out = out;
   a.counters = reinterpret_cast<unsigned int*>(workspace);
   a.parts = reinterpret_cast<float*>(a.counters + kMaxCtas);
