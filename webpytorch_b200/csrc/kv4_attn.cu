@@ -875,7 +875,7 @@ int launch(const AttnArgs& a, int ctas, cudaStream_t st) {
   // single fp16 probability. The host knows the mean only. Measured, 64 requests of 4000 positions, bf16, HD = 128,
   // one plane (two planes): 32 heads over 8, 1 token 103 us (99), 3 tokens 107 (183); over 4, 1 token 62 (58),
   // 2 tokens 66 (100). HD = 256, 32 requests: 32 over 4, 1 token 63.6 (63.4), 2 tokens 80 (101).
-  constexpr bool can = HD != 256 && DT != QL_F32;
+  constexpr bool can = DT != QL_F32;
   if (can && (long)a.T * (a.NH / a.NKV) > 8L * a.B) return launch_one<DT, HD, G, can ? 1 : 2>(a, ctas, st);
   return launch_one<DT, HD, G, 2>(a, ctas, st);
 }
