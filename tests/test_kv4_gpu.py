@@ -205,6 +205,17 @@ def test_cache_codes_bit_exact(dtype, T, NH, NKV, HD, group, page, norm):
         assert np.array_equal(np.isnan(got), np.isnan(ref)) and (got == ref)[~np.isnan(ref)].all()
 
 
+@pytest.mark.parametrize("HD,rot,norm,pad", [(128, 128, False, 0), (128, 128, True, 0), (64, 32, True, 0), (256, 256, True, 0), (128, 128, True, 3)])
+def test_norm_rope_is_the_ieee_steps_to_the_bit(HD, rot, norm, pad):
+    """fp32 outputs equal the definition's steps, none of them fused with another, at sizes where one in a hundred
+    elements would show it."""
+    xt, x, cos, sin, pos, (qw, kw) = rope_case(300, 6, 2, HD, rot, "f32", norm, HD + rot, pad)
+    q, k = kv4.qk_norm_rope(xt, 6, 2, HD, dev(pos), dev(cos), dev(sin), q_weight=wt(qw), k_weight=wt(kw), eps=1e-6)
+    c, s = cos[pos][:, None], sin[pos][:, None]
+    for got, ref in ((q, ok.norm_rotate32(x[:, :6], qw, c, s, 1e-6)), (k, ok.norm_rotate32(x[:, 6:8], kw, c, s, 1e-6))):
+        assert np.array_equal(got.cpu().numpy(), ref)
+
+
 def test_position_past_the_tables_gives_nan_and_is_not_cached():
     xt, _, cos, sin, _, _ = rope_case(2, 2, 1, 64, 64, "f32", False, 1, lmax=8)
     cache = kv4.KV4Cache(1, 1, 64, page=16, group=32)

@@ -7,6 +7,11 @@
 // have to come out the same wherever they are made, so every step is an IEEE operation without
 // contraction and the mean's sum is a balanced tree of neighbours: x0 + x1, (x0 + x1) + (x2 + x3), ...
 // which is what lanes that hold consecutive elements and a butterfly over the lanes add up.
+//
+// A call of many tokens has to read the rows and write q and the codes (430 MB at 16384 tokens of 32 + 8 + 8 heads of
+// 128 in bf16: 66 us at the measured copy rate); the kernel takes 135 us there, 3.2 TB/s: about 190 instructions
+// for 8 elements of a lane, half of them chains (the sum's tree and butterfly, square root and reciprocal, the
+// group's minimum and range), fill half of the issue slots. A call of a few tokens is one launch (6 us).
 #include "kv4_common.cuh"
 
 namespace ql {
@@ -142,19 +147,11 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
     reinterpret_cast<__half2*>(blk + code_bytes(HD))[r * (HD / a.group) + lane / gl] = __halves2half2(s, m);
 }
 
-// Pairs of IEEE fp32 operations in one instruction.
+// Two IEEE fp32 products in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
   asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
       "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
@@ -195,7 +192,9 @@ __device__ __forceinline__ uint32_t round_quotients(const float (&d)[E], float s
 // Rows of 16-byte aligned heads whose rotated halves are whole 16-byte pieces: a lane holds E consecutive
 // elements (16 bytes; 8 fp32 elements at HD = 256), so 16 bytes a lane are read and written, a warp takes
 // 32 E / HD heads at a time, and one token's cos, sin and slot serve all of its heads. `split` warps share a
-// token, so that few tokens still fill the GPU. kAhead loads are under way at once.
+// token, so that few tokens still fill the GPU; with many tokens each warp takes a whole one, since what it does
+// once (position, cos, sin) is 4 us of its 27 (16384 tokens, 1 / 2 / 4 warps a token: 135 / 147 / 177 us). kAhead loads
+// are under way at once. All other rows take the kernel above: 297 us at 16384 tokens, the same time up to 16.
 constexpr int kVecThreads = 256;
 constexpr int kAhead = 4;
 
@@ -358,10 +357,12 @@ __device__ __forceinline__ void heads(const RopeArgs& a, const Token<DT, HD>& k,
         }
 #pragma unroll
         for (int j = 0; j < E; j += 2) {
-          // x c - y s is x c + y (-s) to the bit
+          // x c - y s is x c + y (-s) to the bit. The sums are not packed: ptxas fuses a packed product with a packed
+          // sum, their .rn notwithstanding.
           const float2 y = make_float2(__shfl_sync(0xffffffffu, x[j], k.partner), __shfl_sync(0xffffffffu, x[j + 1], k.partner));
-          const float2 z = add2(mul2(make_float2(x[j], x[j + 1]), make_float2(k.c[j], k.c[j + 1])),
-                                mul2(y, make_float2(k.s[j], k.s[j + 1])));
+          const float2 xc = mul2(make_float2(x[j], x[j + 1]), make_float2(k.c[j], k.c[j + 1]));
+          const float2 ys = mul2(y, make_float2(k.s[j], k.s[j + 1]));
+          const float2 z = make_float2(__fadd_rn(xc.x, ys.x), __fadd_rn(xc.y, ys.y));
           x[j] = FULL || k.turns ? z.x : x[j];
           x[j + 1] = FULL || k.turns ? z.y : x[j + 1];
         }
