@@ -471,6 +471,24 @@ def test_same_inputs_same_bits_on_any_stream():
         assert torch.equal(a, x)
 
 
+def test_queries_that_another_stream_still_writes():
+    """Unaligned queries are copied first: on the call's stream, behind what writes them."""
+    bt = Batch([60, 33], 2, 64, 16, 32, 14)
+    q, cu = bt.queries([1, 1], 4, "bf16")
+    want = attend(bt, q, None)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    wide = torch.zeros((2, 1 + 4 * 64), dtype=torch.bfloat16, device=DEV)
+    qs = wide[:, 1:].unflatten(1, (4, 64))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)
+        qs.copy_(q)
+    got = attend(bt, qs, None, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_step_in_a_graph():
     """plan, write and attention captured once and replayed with new inputs."""
     rng = np.random.default_rng(3)

@@ -66,29 +66,31 @@ class KV4Cache:
 
     def read(self, slots, stream=None):
         """(k, v) fp16 [T, NKV, HD]: the values that slots int64 [T] stand for; zeros for -1."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.read(slots)
         _need(slots, "slots", torch.int64, 1)
         T = slots.shape[0]
         k, v = slots.new_empty((2, T, self.NKV, self.HD), dtype=torch.float16).unbind(0)
         _ffi.call("ql_kv4_read", self.data.data_ptr(), self.num_pages, self.NKV, self.HD, self.page, self.group,
-                  slots.data_ptr(), T, k.data_ptr(), v.data_ptr(), _ffi.stream_ptr(stream, self.device))
+                  slots.data_ptr(), T, k.data_ptr(), v.data_ptr(), _ffi.stream_ptr(None, self.device))
         return k, v
 
 
 _workspaces = {}
 
 
-def _attention_workspace(cache, NH, stream):
-    """The attention's workspace on this stream, made once and shared by the layers' caches: its counters
+def _attention_workspace(cache, NH):
+    """The attention's workspace on the current stream, made once and shared by the layers' caches: its counters
     are zero between calls, and calls that share one may not overlap."""
-    key = (cache.device.index, cache.HD, _ffi.stream_ptr(stream, cache.device))
+    key = (cache.device.index, cache.HD, _ffi.stream_ptr(None, cache.device))
     ws = _workspaces.get(key)
     if ws is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("attention needs its workspace before a graph is captured: call it once on this "
                                "stream first, or pass workspace=")
         n = int(_ffi.fn("ql_kv4_attention_workspace")(NH, cache.NKV, cache.HD))
-        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(cache.device)):
-            ws = _workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=cache.device)
+        ws = _workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=cache.device)
     return ws
 
 
@@ -101,6 +103,9 @@ def plan(prev_lens, new_lens, block_table, free_pages, n_free, page, max_tokens,
     as new tensors. Requests are served first come first served, as far as max_tokens and the free
     pages go; one that is not keeps its length. Returns Plan(seq_lens, cu_new [n + 1], slots, positions,
     requests [max_tokens], n_free); entries past cu_new[n] are -1."""
+    if stream is not None:
+        with torch.cuda.stream(stream):              # what is allocated here belongs to it too
+            return plan(prev_lens, new_lens, block_table, free_pages, n_free, page, max_tokens)
     _need(prev_lens, "prev_lens", torch.int32, 1)
     _need(new_lens, "new_lens", torch.int32, 1)
     _need(block_table, "block_table", torch.int32, 2)
@@ -119,7 +124,7 @@ def plan(prev_lens, new_lens, block_table, free_pages, n_free, page, max_tokens,
               block_table.stride(0) if n > 1 else width, width, free_pages.data_ptr(), free_pages.shape[0],
               n_free.data_ptr(), page, max_tokens, lens.data_ptr(), cu.data_ptr(), slots.data_ptr(), pos.data_ptr(),
               req.data_ptr(), left.data_ptr(), ws.data_ptr() if ws_ints else None, 4 * ws_ints,
-              _ffi.stream_ptr(stream, prev_lens.device))
+              _ffi.stream_ptr(None, prev_lens.device))
     return Plan(lens, cu, slots, pos, req, left)
 
 
@@ -130,6 +135,10 @@ def qk_norm_rope(qkv, NH, NKV, HD, positions, cos, sin, *, q_weight=None, k_weig
     [lmax, rot / 2]. With a cache, keys and values are quantised into its slots int64 [T] and (q, None)
     comes back, without one (q, k); q [T, NH, HD], k [T, NKV, HD] in qkv's dtype. A negative position is
     padding."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return qk_norm_rope(qkv, NH, NKV, HD, positions, cos, sin, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                cache=cache, slots=slots, out=out)
     _need(qkv, "qkv", qkv.dtype, 2)
     T, width = qkv.shape
     if width != (NH + 2 * NKV) * HD:
@@ -160,7 +169,7 @@ def qk_norm_rope(qkv, NH, NKV, HD, positions, cos, sin, *, q_weight=None, k_weig
         where = (None, cache.data.data_ptr(), cache.num_pages, cache.page, cache.group, slots.data_ptr())
     _ffi.call("ql_qk_norm_rope", qkv.data_ptr(), _ffi.dtype_code(qkv.dtype), qkv.stride(0) if T > 1 else width, T, NH, NKV,
               HD, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), lmax, 2 * half, _ffi.ptr(q_weight),
-              _ffi.ptr(k_weight), eps, out.data_ptr(), *where, _ffi.stream_ptr(stream, qkv.device))
+              _ffi.ptr(k_weight), eps, out.data_ptr(), *where, _ffi.stream_ptr(None, qkv.device))
     return out, k
 
 
@@ -174,6 +183,9 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
     (0: all). workspace: uint8 of ql_kv4_attention_workspace bytes, zeroed once and not shared by calls that
     overlap (None: one for each stream). Rows that see nothing, and rows past cu_q[B], are zero. Returns
     [T, NH, HD] in q's dtype."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return attention(q, cache, block_table, seq_lens, cu_q, scale=scale, window=window, out=out, workspace=workspace)
     _need(q, "q", q.dtype, 3)
     T, NH, HD = q.shape
     ldq = NH * HD
@@ -201,9 +213,9 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
         out = torch.empty_like(q) if dense else q.new_empty((T, NH, HD))
     elif out.dtype != q.dtype or tuple(out.shape) != (T, NH, HD) or not out.is_contiguous():
         raise ValueError("out must be a contiguous %s tensor %s" % (q.dtype, (T, NH, HD)))
-    ws = _attention_workspace(cache, NH, stream) if workspace is None else workspace
+    ws = _attention_workspace(cache, NH) if workspace is None else workspace
     _ffi.call("ql_kv4_attention", q.data_ptr(), _ffi.dtype_code(q.dtype), ldq, T, NH, cache.NKV, HD, cache.data.data_ptr(),
               cache.num_pages, cache.page, cache.group, block_table.data_ptr(), block_table.stride(0) if B > 1 else width,
               width, seq_lens.data_ptr(), _ffi.ptr(cu_q), B, HD ** -0.5 if scale is None else scale, window,
-              out.data_ptr(), ws.data_ptr(), ws.numel(), _ffi.stream_ptr(stream, q.device))
+              out.data_ptr(), ws.data_ptr(), ws.numel(), _ffi.stream_ptr(None, q.device))
     return out
