@@ -6,13 +6,18 @@
 // sums over the requests that fit their table row, avail = free pages + pages given back. Both sums
 // grow with b, so the served requests that need pages are the first ones that do, and the pages
 // taken are a contiguous piece of the stack, from its top.
+//
+// The work is a launch and two dependent block scans; the bytes (4.3 MB of maps at 262144 tokens) are under a
+// microsecond. 8 requests take 5 us, 1000 with 20000 tokens 9, 6000 with 262144 tokens 18 (lengths staged in
+// shared memory first: the same).
 #include "ql_common.cuh"
 
 namespace ql {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kMost = 16384;   // requests whose sums fit in shared memory
+// Requests whose sums fit in shared memory (16384 requests 68 us there, 16385 in the workspace 79).
+constexpr int kMost = 16384;
 
 struct PlanArgs {
   const int32_t* prev;

@@ -1,6 +1,6 @@
-// Attention of prompt chunks over the paged 4-bit cache on the 5th-generation tensor cores: fp16 or
-// bf16 queries of a request that fill kPromptRows rows (query tokens x heads of a key/value head) or
-// more, HD 64 or 128. The other requests of a call are the streaming kernel's.
+// Attention of prompt chunks over the paged 4-bit cache on the 5th-generation tensor cores: requests with
+// kPromptRows rows (query tokens x heads of a key/value head) or more of fp16 or bf16 queries, HD 64 or 128, in calls
+// with enough of them. The other requests of a call are the streaming kernel's.
 //
 // A CTA takes two tiles of 128 rows of one request and key/value head and walks the positions they see
 // in steps of 128:
@@ -18,6 +18,10 @@
 // the same layout read as MN-major for P V. The order of a position's elements is free (the contraction of
 // S; the columns of O), so it is the one in which a lane's 16-byte load of 32 codes gives four 16-byte
 // stores without bank conflicts.
+// Bound. 4 NH HD operations a visible (query, position): 93.5 us at the measured rate for two chunks of 900 to 2000
+// tokens over 2500 to 6000 positions (32 heads over 4, HD 128, bf16), which take 259 us, 600 TFLOP/s. A step of
+// 128 positions takes a CTA 2.2 us: one exponential a score and the decoding of the codes fill the issue slots
+// beside the tensor work, and 370 pairs of tiles over 148 SMs leave the last wave half empty.
 #include "kv4_common.cuh"
 #include "kv4_attn.cuh"
 #include "sm100_ptx.cuh"
@@ -434,9 +438,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     if (!ok)                                       // no copy is left in flight
       for (int k = n; k < min(issued, mine); ++k) ptx::mbar_wait_drain(bar + 8 * (k % kRing), (k / kRing) & 1);
   } else if (steps > 0) {
-    // ---------------- MMA issue: the warp runs converged, one lane issues, and what the MMAs take is the
-    // same for all lanes by construction, which keeps
-    // descriptors in uniform registers: about 110 cycles an MMA without, against 64 of tensor work
+    // ---------------- MMA issue: the warp runs converged, one lane issues, and what the MMAs take is the same
+    // for all lanes by construction, which keeps descriptors in uniform registers (an MMA takes about 110 cycles to
+    // issue without, against 64 of tensor work)
     constexpr uint32_t kIdescS = ptx::idesc_f16_f32(128, kHalf);
     constexpr uint32_t kIdescO = ptx::idesc_f16_f32(128, HD) | ptx::kIdescBMn;
     volatile int* ab = const_cast<volatile int*>(abort_flag);

@@ -8,10 +8,10 @@
 // contraction and the mean's sum is a balanced tree of neighbours: x0 + x1, (x0 + x1) + (x2 + x3), ...
 // which is what lanes that hold consecutive elements and a butterfly over the lanes add up.
 //
-// A call of many tokens has to read the rows and write q and the codes (430 MB at 16384 tokens of 32 + 8 + 8 heads of
-// 128 in bf16: 66 us at the measured copy rate); the kernel takes 135 us there, 3.2 TB/s: about 190 instructions
-// for 8 elements of a lane, half of them chains (the sum's tree and butterfly, square root and reciprocal, the
-// group's minimum and range), fill half of the issue slots. A call of a few tokens is one launch (6 us).
+// A call of many tokens has to read the rows and write q and the codes: 363 MB at 16384 tokens of 32 + 8 + 8 heads
+// of 128 in bf16, 55 us at the measured copy rate. The kernel takes 112 us there, 3.2 TB/s: about 190
+// instructions for 8 elements of a lane, many of them chains (the sum's tree and butterfly, square root and
+// reciprocal, the group's minimum and range), fill 68 % of the issue slots. A call of a few tokens is one launch (6 us).
 #include "kv4_common.cuh"
 
 namespace ql {
@@ -193,8 +193,9 @@ __device__ __forceinline__ uint32_t round_quotients(const float (&d)[E], float s
 // elements (16 bytes; 8 fp32 elements at HD = 256), so 16 bytes a lane are read and written, a warp takes
 // 32 E / HD heads at a time, and one token's cos, sin and slot serve all of its heads. `split` warps share a
 // token, so that few tokens still fill the GPU; with many tokens each warp takes a whole one, since what it does
-// once (position, cos, sin) is 4 us of its 27 (16384 tokens, 1 / 2 / 4 warps a token: 135 / 147 / 177 us). kAhead loads
-// are under way at once. All other rows take the kernel above: 297 us at 16384 tokens, the same time up to 16.
+// once (position, cos, sin) is 4 us of its 27 (16384 tokens with the read of what was written, 1 / 2 / 4 warps a token:
+// 135 / 147 / 177 us). kAhead loads are under way at once. All other rows take the kernel above: 297 us there, the
+// same time up to 16 tokens.
 constexpr int kVecThreads = 256;
 constexpr int kAhead = 4;
 
