@@ -339,6 +339,7 @@ def test_prompts(dtype, HD, NH, NKV, page, group, lens, ql, window):
     (128, 40, 8, 32, 32, [1, 257, 128], [1, 193, 13]), (128, 8, 8, 16, 64, [900], [800]), (64, 64, 4, 32, 32, [257, 90, 260], [150, 1, 129]),
     (64, 16, 16, 16, 64, [1000], [800]), (64, 14, 2, 64, 32, [1023, 64], [900, 1]), (256, 16, 2, 16, 64, [333, 20], [200, 20]),
     (256, 16, 2, 32, 32, [70, 129, 5], [20, 129, 1]), (256, 40, 8, 16, 128, [400], [60]),
+    (64, 32, 32, 16, 32, [700], [600]), (128, 16, 16, 16, 64, [300, 1200], [70, 1030]), (128, 32, 4, 64, 64, [2500, 100], [300, 9]),
 ])
 @pytest.mark.parametrize("window", [0, 1, 130])
 def test_many_rows(dtype, HD, NH, NKV, page, group, lens, ql, window):

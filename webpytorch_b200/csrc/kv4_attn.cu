@@ -839,13 +839,13 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
 }
 
 // Whether requests of kPromptRows rows or more are the prompt kernel's. It takes 16 positions of 16 rows in a
-// fifth of the streaming kernel's time (0.16 against 0.8 ns at HD = 128), but walks the positions of 256 rows in
-// one CTA, 17 ns each, where the streaming kernel cuts them over all: at rows x heads / 256 x 0.8 ns a position
-// the two are level whatever the length. The host knows the tokens past one a request. Measured, both sides,
-// bf16, 32 heads over 4, 6000 positions: 128 query tokens 118 us (streaming 85), 256 119 (148), 2000 204 (1014);
-// 8 x 17 tokens over 3000 66 (60), 8 x 32 70 (87); 16 heads of 64, 3000 positions: 256 tokens 59 (35), 1000 60 (84).
+// fifth of the streaming kernel's time (0.16 against 0.8 ns over all SMs at HD = 128), and costs a join and another
+// launch, so it pays from some rows on. The host knows the tokens past one a request. Measured, both sides,
+// bf16: 32 heads of 128 over 4, 6000 positions, 17 tokens 31 us (streaming 32), 32 35 (38), 64 35 (53), 256 48 (151), 2000
+// 204 (1014); 64 tokens over 64 positions 21 (18), over 1000 27 (28); 8 requests of 8 tokens 35 (37), of 32 48 (90); 16
+// heads of 64, 3000 positions: 64 tokens 25 (23), 256 32 (35).
 bool prompts_pay(int T, int B, int NH, int HD, int dtype) {
-  return dtype != QL_F32 && HD <= 128 && (long)(T - B) * NH * HD >= 3l << 18;
+  return dtype != QL_F32 && HD <= 128 && (long)(T - B) * NH * HD >= 1l << 17;
 }
 
 int sm_count() {
@@ -859,8 +859,10 @@ template <int HD>
 constexpr size_t part_floats() {
   return (size_t)(2 + Shape<HD>::kWarps) * Part<HD, 1>::kFloats;
 }
+// The two kernels run one after the other and share the memory.
 size_t parts_bytes(int HD, int ctas) {
-  return (HD == 64 ? part_floats<64>() : HD == 128 ? part_floats<128>() : part_floats<256>()) * ctas * sizeof(float);
+  const size_t own = (HD == 64 ? part_floats<64>() : HD == 128 ? part_floats<128>() : part_floats<256>()) * ctas * sizeof(float);
+  return max(own, kv4_prompt_bytes(HD, ctas));
 }
 
 template <int DT, int HD, int G, int PL>
@@ -976,7 +978,7 @@ extern "C" int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int N
   a.parts = reinterpret_cast<float*>(a.counters + kMaxCtas);
   const cudaStream_t st = (cudaStream_t)stream;
   if (a.prompt_rows && cu_q) {
-    const int rc = kv4_prompt_attention(a, dtype, HD, group, st);
+    const int rc = kv4_prompt_attention(a, dtype, HD, group, ctas, st);
     if (rc) return rc;
   } else {
     a.prompt_rows = 0;

@@ -56,7 +56,9 @@ __device__ __forceinline__ void issue(const AttnArgs& a, uint32_t src, int stage
 }  // namespace kv4
 
 // Requests of kPromptRows rows or more, 16-bit types, HD 64 or 128 (kv4_prompt.cu).
-int kv4_prompt_attention(const kv4::AttnArgs& a, int dtype, int HD, int group, cudaStream_t st);
+// Calls of few rows leave parts in a.parts, kv4_prompt_bytes of it, for a GPU of `ctas` SMs.
+int kv4_prompt_attention(const kv4::AttnArgs& a, int dtype, int HD, int group, int ctas, cudaStream_t st);
+size_t kv4_prompt_bytes(int HD, int ctas);
 int take_kv4_prompt_status();
 
 }  // namespace ql

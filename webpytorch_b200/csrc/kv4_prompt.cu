@@ -36,6 +36,7 @@ using namespace kv4;
 
 constexpr int kTileRows = 128, kTiles = 2, kStep = 128, kHalf = kStep / 2;
 constexpr int kSoftWarps = 8, kDecodeWarps = 4, kWarps = kSoftWarps + kDecodeWarps + 1, kThreads = kWarps * 32;
+constexpr int kMostSplits = 16;                 // pieces of a pair's positions
 constexpr int kRing = 3;                        // blocks of a decoding warp in flight
 
 template <int HD, int G>
@@ -172,29 +173,63 @@ __device__ __forceinline__ bool softmax_half(Row& row, uint32_t s_col, uint32_t 
   return true;
 }
 
-template <int DT, int HD, int G>
+constexpr int kRows = kTiles * kTileRows;
+
+// Pair of tiles `item` of `items`, tiles of the longest rows first: rows r0 .. r0 + nrows - 1 of request b and a
+// key/value head. nrows is 0 for one past a request's last row, or of a request that is not the prompt kernel's.
+struct Item {
+  int b, kvh, q0, ql, r0, nrows;
+};
+__device__ __forceinline__ Item item_at(const AttnArgs& a, int grp, int item, int items) {
+  Item it;
+  it.kvh = item % a.NKV;
+  const int x = items / a.NKV - 1 - item / a.NKV;
+  const auto tile_start = [&](int b) { return (int)((long)cu(a, b) * grp / kRows) + b; };
+  it.b = 0;
+  for (int hi = a.B - 1; it.b < hi;) {            // the last request whose first pair of tiles is at or before x
+    const int mid = (it.b + hi + 1) >> 1;
+    if (tile_start(mid) <= x) it.b = mid;
+    else hi = mid - 1;
+  }
+  it.q0 = cu(a, it.b);
+  it.ql = max(cu(a, it.b + 1) - it.q0, 0);
+  const int rows = it.ql * grp;
+  it.r0 = (x - tile_start(it.b)) * kRows;
+  it.nrows = rows < a.prompt_rows || it.r0 >= rows ? 0 : min(kRows, rows - it.r0);
+  return it;
+}
+
+// A part of a pair of tiles: HD / 4 x kRows fours of O (a row's four to a lane, so that lanes store and load next
+// to each other), then (m, l) of the rows.
+template <int HD>
+constexpr int part_floats() { return kRows * (HD + 2); }
+template <int HD>
+__device__ __forceinline__ float* part_of(const AttnArgs& a, int split, int item, int items) {
+  return a.parts + ((long)split * items + item) * part_floats<HD>();
+}
+
+// CUT: where a call has at most half as many pairs of tiles as the GPU has SMs, the positions of a pair are cut
+// into gridDim.y equal pieces, and prompt_join_kernel adds up what they leave. (256 tokens over 6000 positions, 32
+// heads over 4: 119 us whole, 47 cut; 64 tokens 117 and 34. One kernel for both took 266 us where the whole
+// one takes 260.)
+template <int DT, int HD, int G, bool CUT>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
   using L = Smem<HD, G>;
   constexpr int BB = block_bytes(HD, G), W = HD / 8;
   const int grp = a.NH / a.NKV;
-  // tiles of the longest rows first
-  const int kvh = blockIdx.x % a.NKV, x = gridDim.x / a.NKV - 1 - blockIdx.x / a.NKV;
-  constexpr int kRows = kTiles * kTileRows;
-  const auto tile_start = [&](int b) { return (int)((long)cu(a, b) * grp / kRows) + b; };
-  int b = 0;
-  for (int hi = a.B - 1; b < hi;) {               // the last request whose first pair of tiles is at or before x
-    const int mid = (b + hi + 1) >> 1;
-    if (tile_start(mid) <= x) b = mid;
-    else hi = mid - 1;
-  }
-  const int q0 = cu(a, b), ql = max(cu(a, b + 1) - q0, 0), rows = ql * grp, r0 = (x - tile_start(b)) * kRows;
-  if (rows < a.prompt_rows || r0 >= rows) return;
-  const int nrows = min(kRows, rows - r0);
+  const Item item = item_at(a, grp, blockIdx.x, gridDim.x);
+  if (item.nrows == 0) return;
+  const int b = item.b, kvh = item.kvh, q0 = item.q0, ql = item.ql, r0 = item.r0, nrows = item.nrows;
   const int seq = max(a.seq_lens[b], 0), table_end = a.width << a.page_shift;
   const int p_first = seq - ql + r0 / grp, p_last = seq - ql + (r0 + nrows - 1) / grp;
   const int lo_all = a.window ? max(p_first - a.window + 1, 0) : 0, hi_all = min(p_last + 1, table_end);
-  const int blk0 = lo_all / kBlock, nblk = max((hi_all + kBlock - 1) / kBlock - blk0, 0);
-  const int steps = (nblk + kStep / kBlock - 1) / (kStep / kBlock);
+  constexpr int kStepBlocks = kStep / kBlock;
+  const int blk_lo = lo_all / kBlock, blk_all = max((hi_all + kBlock - 1) / kBlock - blk_lo, 0);
+  const int all_steps = (blk_all + kStepBlocks - 1) / kStepBlocks;
+  const int each = CUT ? (all_steps + gridDim.y - 1) / gridDim.y : all_steps;
+  const int first_step = CUT ? min((int)blockIdx.y * each, all_steps) : 0, steps = min(each, all_steps - first_step);
+  const int blk0 = blk_lo + first_step * kStepBlocks;
+  const int nblk = CUT ? min(blk_all - first_step * kStepBlocks, steps * kStepBlocks) : blk_all;
 
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -309,7 +344,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     if (steps > 0 && ok) ok = warp_wait(done, 0, ab);
     ptx::tc_fence_after();
     if (*bad_flag || !ok) run.l = __int_as_float(0x7fc00000);
-    const float inv = run.l == 0.f ? 0.f : 1.f / run.l;   // a row that sees nothing is zero
+    const float inv = CUT ? 1.f : run.l == 0.f ? 0.f : 1.f / run.l;   // a row that sees nothing is zero
+    float4* part = CUT ? reinterpret_cast<float4*>(part_of<HD>(a, blockIdx.y, blockIdx.x, gridDim.x)) : nullptr;
+    if (CUT) reinterpret_cast<float2*>(part + HD / 4 * kRows)[i] = make_float2(run.m, run.l);
     uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + ((long)tok * a.NH + head) * HD;
 #pragma unroll
     for (int k = 0; k < HD / 32; ++k) {
@@ -322,24 +359,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
       for (int c = 0; c < 4; ++c) {               // columns 8 (4 k + c) ...: one word's elements
         const int pc = 4 * k + c, panel = pc >> 3, col = pc & 7;
         const int w = HD == 64 ? pc : 4 * (col >> 1) + 2 * panel + (col & 1);
-        uint32_t o[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          // element e of the word is at 2 e, elements 4 + e at 2 e + 1
-          const int e0 = 2 * q, e1 = 2 * q + 1;
-          const float y0 = steps > 0 ? __uint_as_float(v[8 * c + (e0 < 4 ? 2 * e0 : 2 * (e0 - 4) + 1)]) * inv : 0.f * inv;
-          const float y1 = steps > 0 ? __uint_as_float(v[8 * c + (e1 < 4 ? 2 * e1 : 2 * (e1 - 4) + 1)]) * inv : 0.f * inv;
-          if (DT == QL_F16) {
-            o[q] = h2_as_u32(__floats2half2_rn(y0, y1));
-          } else {
-            const __nv_bfloat162 t = __floats2bfloat162_rn(y0, y1);
-            o[q] = *reinterpret_cast<const uint32_t*>(&t);
+        if constexpr (CUT) {
+          if (steps > 0) {
+            const auto f = [&](int e) { return __uint_as_float(v[8 * c + e]); };   // elements (0, 4), (1, 5), (2, 6), (3, 7)
+            part[(2 * w) * kRows + i] = make_float4(f(0), f(2), f(4), f(6));
+            part[(2 * w + 1) * kRows + i] = make_float4(f(1), f(3), f(5), f(7));
           }
-        }
-        if (live) {
-          uint2* to = reinterpret_cast<uint2*>(out + 8 * w);
-          to[0] = make_uint2(o[0], o[1]);
-          to[1] = make_uint2(o[2], o[3]);
+        } else {
+          uint32_t o[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            // element e of the word is at 2 e, elements 4 + e at 2 e + 1
+            const int e0 = 2 * q, e1 = 2 * q + 1;
+            const float y0 = steps > 0 ? __uint_as_float(v[8 * c + (e0 < 4 ? 2 * e0 : 2 * (e0 - 4) + 1)]) * inv : 0.f * inv;
+            const float y1 = steps > 0 ? __uint_as_float(v[8 * c + (e1 < 4 ? 2 * e1 : 2 * (e1 - 4) + 1)]) * inv : 0.f * inv;
+            if (DT == QL_F16) {
+              o[q] = h2_as_u32(__floats2half2_rn(y0, y1));
+            } else {
+              const __nv_bfloat162 t = __floats2bfloat162_rn(y0, y1);
+              o[q] = *reinterpret_cast<const uint32_t*>(&t);
+            }
+          }
+          if (live) {
+            uint2* to = reinterpret_cast<uint2*>(out + 8 * w);
+            to[0] = make_uint2(o[0], o[1]);
+            to[1] = make_uint2(o[2], o[3]);
+          }
         }
       }
     }
@@ -518,9 +563,59 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
   if (warp == kWarps - 1) ptx::tmem_dealloc(tmem, 512);
 }
 
-template <int DT, int HD, int G>
-int launch(const AttnArgs& a, cudaStream_t st) {
-  auto kern = kv4_prompt_kernel<DT, HD, G>;
+// Rows of pairs of tiles whose positions were cut: O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s, in the order of
+// the pieces. A thread has 32 elements of a row.
+template <int DT, int HD>
+__global__ void __launch_bounds__(kRows) prompt_join_kernel(AttnArgs a, int splits) {
+  const int grp = a.NH / a.NKV, i = threadIdx.x;
+  const Item item = item_at(a, grp, blockIdx.x, gridDim.x);
+  if (i >= item.nrows) return;
+  const auto part = [&](int s) { return reinterpret_cast<const float4*>(part_of<HD>(a, s, blockIdx.x, gridDim.x)); };
+  const auto stats = [&](int s) { return reinterpret_cast<const float2*>(part(s) + HD / 4 * kRows)[i]; };
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, stats(s).x);
+  float4 acc[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < splits; ++s) {
+    const float2 ml = stats(s);
+    if (ml.x == -INFINITY) {                      // nothing seen, and O may not have been written; l is 0 or nan
+      l += ml.y;
+      continue;
+    }
+    const float f = ex2(ml.x - m);
+    l = fmaf(f, ml.y, l);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const float4 v = part(s)[(8 * blockIdx.y + c) * kRows + i];
+      acc[c].x = fmaf(f, v.x, acc[c].x);
+      acc[c].y = fmaf(f, v.y, acc[c].y);
+      acc[c].z = fmaf(f, v.z, acc[c].z);
+      acc[c].w = fmaf(f, v.w, acc[c].w);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;     // a row that sees nothing is zero
+  const int row = item.r0 + i;
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) +
+                  ((long)(item.q0 + row / grp) * a.NH + item.kvh * grp + row % grp) * HD + 32 * blockIdx.y;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint2 o;
+    if (DT == QL_F16) {
+      o = make_uint2(h2_as_u32(__floats2half2_rn(acc[c].x * inv, acc[c].y * inv)),
+                     h2_as_u32(__floats2half2_rn(acc[c].z * inv, acc[c].w * inv)));
+    } else {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(acc[c].x * inv, acc[c].y * inv);
+      const __nv_bfloat162 y = __floats2bfloat162_rn(acc[c].z * inv, acc[c].w * inv);
+      o = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+    reinterpret_cast<uint2*>(out)[c] = o;
+  }
+}
+
+template <int DT, int HD, int G, bool CUT>
+int launch_one(const AttnArgs& a, dim3 grid, cudaStream_t st) {
+  auto kern = kv4_prompt_kernel<DT, HD, G, CUT>;
   static int configured_dev = -1;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -530,23 +625,37 @@ int launch(const AttnArgs& a, cudaStream_t st) {
     if (rc) return rc;
     configured_dev = dev;
   }
-  const long pairs = (long)a.T * (a.NH / a.NKV) / (kTiles * kTileRows) + a.B;
-  kern<<<(unsigned)(pairs * a.NKV), kThreads, Smem<HD, G>::kBytes, st>>>(a);
+  kern<<<grid, kThreads, Smem<HD, G>::kBytes, st>>>(a);
   return cuda_status(cudaGetLastError(), "ql_kv4_attention (prompt) launch");
 }
 
+template <int DT, int HD, int G>
+int launch(const AttnArgs& a, int ctas, cudaStream_t st) {
+  const long items = ((long)a.T * (a.NH / a.NKV) / kRows + a.B) * a.NKV;
+  const int splits = (int)max(1L, min(ctas / items, (long)kMostSplits));
+  if (splits == 1) return launch_one<DT, HD, G, false>(a, dim3((unsigned)items), st);
+  const int rc = launch_one<DT, HD, G, true>(a, dim3((unsigned)items, splits), st);
+  if (rc) return rc;
+  prompt_join_kernel<DT, HD><<<dim3((unsigned)items, HD / 32), kRows, 0, st>>>(a, splits);
+  return cuda_status(cudaGetLastError(), "ql_kv4_attention (prompt join) launch");
+}
+
 template <int DT>
-int launch_sizes(const AttnArgs& a, int HD, int group, cudaStream_t st) {
-  if (HD == 64) return group == 32 ? launch<DT, 64, 32>(a, st) : launch<DT, 64, 64>(a, st);
-  return group == 32   ? launch<DT, 128, 32>(a, st)
-         : group == 64 ? launch<DT, 128, 64>(a, st)
-                       : launch<DT, 128, 128>(a, st);
+int launch_sizes(const AttnArgs& a, int HD, int group, int ctas, cudaStream_t st) {
+  if (HD == 64) return group == 32 ? launch<DT, 64, 32>(a, ctas, st) : launch<DT, 64, 64>(a, ctas, st);
+  return group == 32   ? launch<DT, 128, 32>(a, ctas, st)
+         : group == 64 ? launch<DT, 128, 64>(a, ctas, st)
+                       : launch<DT, 128, 128>(a, ctas, st);
 }
 
 }  // namespace
 
-int kv4_prompt_attention(const AttnArgs& a, int dtype, int HD, int group, cudaStream_t st) {
-  return dtype == QL_F16 ? launch_sizes<QL_F16>(a, HD, group, st) : launch_sizes<QL_BF16>(a, HD, group, st);
+size_t kv4_prompt_bytes(int HD, int ctas) {
+  return (size_t)ctas * (HD == 64 ? part_floats<64>() : HD == 128 ? part_floats<128>() : 0) * sizeof(float);
+}
+
+int kv4_prompt_attention(const AttnArgs& a, int dtype, int HD, int group, int ctas, cudaStream_t st) {
+  return dtype == QL_F16 ? launch_sizes<QL_F16>(a, HD, group, ctas, st) : launch_sizes<QL_BF16>(a, HD, group, ctas, st);
 }
 
 int take_kv4_prompt_status() {
