@@ -136,12 +136,17 @@ def call(name, *args):
     return rc
 
 
+_dtype_codes = {}
+
+
 def dtype_code(t):
-    import torch
-    m = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if t not in m:
+    if not _dtype_codes:
+        import torch
+        _dtype_codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    code = _dtype_codes.get(t)
+    if code is None:
         raise TypeError("unsupported dtype %s (float32, float16 or bfloat16)" % t)
-    return m[t]
+    return code
 
 
 def ptr(t):
