@@ -628,14 +628,15 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
       }
       const bool both = i + 1 < n;
       const int s1 = s + 1 == ST ? 0 : s + 1;
-      if (!ptx::mbar_wait(bar + 8 * s, phase, &abort_flag) ||
-          (both && !ptx::mbar_wait(bar + 8 * s1, phase ^ (s1 == 0), &abort_flag))) {
+      if (!warp_wait(bar + 8 * s, phase, &abort_flag) ||
+          (both && !warp_wait(bar + 8 * s1, phase ^ (s1 == 0), &abort_flag))) {
         // gave up: nan for this tile, and no copy left in flight
         bad = true;
         for (int j = i; j < min(i + ST, n); ++j) {
           ptx::mbar_wait_drain(bar + 8 * s, phase);
           if (++s == ST) s = 0, phase ^= 1;
         }
+        __syncwarp();
         break;
       }
       // a page that is not one of the cache's: nan

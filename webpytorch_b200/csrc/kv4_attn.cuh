@@ -30,6 +30,14 @@ struct AttnArgs {
 
 __device__ __forceinline__ int cu(const AttnArgs& a, int b) { return a.cu_q ? min(max(a.cu_q[b], 0), a.T) : min(b, a.T); }
 
+// A wait by a whole warp. The lanes leave the polling loop at different times, and one may give up on what another
+// still saw complete: the vote brings the warp together, as the tensor-core instructions that follow want it, and
+// makes the answer the same for all lanes.
+template <bool SLEEP = false>
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, SLEEP ? ptx::mbar_wait_sleep(bar, parity, abort_flag) : ptx::mbar_wait(bar, parity, abort_flag));
+}
+
 constexpr uint32_t kNoBlock = 0xffffffffu;
 
 // Block i of n from blk0 of request b, as its index in the cache; kNoBlock past the end or for a page

@@ -67,13 +67,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A wait by a whole warp. The lanes leave the polling loop at different times, and the tensor-memory
-// instructions that follow want the warp converged: the vote brings it together, and the answer is the same
-// for all lanes.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag));
-}
-
 // Pairs of fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -417,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
       // both of this step's blocks arrive, keys first
 #pragma unroll
       for (int kv = 0; kv < 2 && ok; ++kv) {
-        if (!ptx::mbar_wait_sleep(kv ? v_free(st) : k_free(st), par ^ 1, const_cast<volatile int*>(abort_flag))) {
+        if (!warp_wait<true>(kv ? v_free(st) : k_free(st), par ^ 1, const_cast<volatile int*>(abort_flag))) {
           ok = false;
           break;
         }
@@ -433,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
               }
               next = lookup(bn + 32 + lane);
             }
-            if (!ptx::mbar_wait(bar + 8 * (bn % kRing), (bn / kRing) & 1, const_cast<volatile int*>(abort_flag))) {
+            if (!warp_wait(bar + 8 * (bn % kRing), (bn / kRing) & 1, const_cast<volatile int*>(abort_flag))) {
               ok = false;
               break;
             }
@@ -475,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
             issue_one(bn);
           }
         }
+        if (!ok) break;                            // what was not decoded is not handed on
         ptx::fence_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(kv ? v_full(st) : k_full(st));
@@ -505,8 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
       }
       __syncwarp();
     };
-    bool ok = ptx::mbar_wait(q_full, 0, ab) && ptx::mbar_wait(k_full(0), 0, ab);
-    ok = __all_sync(0xffffffffu, ok);
+    bool ok = warp_wait(q_full, 0, ab) && warp_wait(k_full(0), 0, ab);
     ptx::tc_fence_after();
     if (ok) {
 #pragma unroll
@@ -521,12 +514,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
 #pragma unroll
       for (int hi = 0; hi < 2 * kTiles; ++hi) {
         const int h = hi >> 1, i = hi & 1;
-        bool go = ptx::mbar_wait(p_full(i, h), j & 1, ab);
-        if (hi == 0) {
-          go = go && ptx::mbar_wait(v_full(st), par, ab);
-          if (j + 1 < steps) go = go && ptx::mbar_wait(k_full(st1), par1, ab);
-        }
-        ok = ok && __all_sync(0xffffffffu, go);
+        ok = warp_wait(p_full(i, h), j & 1, ab);
+        if (hi == 0) ok = ok && warp_wait(v_full(st), par, ab) && (j + 1 == steps || warp_wait(k_full(st1), par1, ab));
         if (!ok) break;
         ptx::tc_fence_after();
         const uint64_t vd = v_desc + (uint32_t)((st * L::kTile + h * kHalf * 128) >> 4);
