@@ -14,7 +14,8 @@ A step of a batch:
     o = kv4.attention(q, cache, table, p.seq_lens, p.cu_new)                 # each layer
 
 Every call is asynchronous on the current stream (or `stream`), without a host read of any length,
-so a step can be captured in a CUDA graph.
+so a step can be captured in a CUDA graph. All tensors of a call are on the current GPU (that of `stream`, where it
+is given); others are refused.
 """
 from collections import namedtuple
 
@@ -28,18 +29,29 @@ __all__ = ["KV4Cache", "Plan", "plan", "qk_norm_rope", "attention"]
 Plan = namedtuple("Plan", "seq_lens cu_new slots positions requests n_free")
 
 
-def _need(t, name, dtype, dim):
-    """t is a GPU tensor of this type and number of dimensions, its last one contiguous."""
-    if type(t) is torch.Tensor and t.dtype is dtype and t.is_cuda and t.dim() == dim and (
+def _need(t, name, dtype, dim, dev):
+    """t is a tensor of this type and number of dimensions on GPU `dev` (the current one, which the kernels are
+    launched on), its last dimension contiguous."""
+    if type(t) is torch.Tensor and t.dtype is dtype and t.get_device() == dev and t.dim() == dim and (
             t.is_contiguous() or t.stride(-1) == 1):
         return                                     # the calls take a few microseconds: keep this short
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != dim:
         raise TypeError("%s must be a %d-D %s tensor, got %s" % (
             name, dim, dtype, "%s %s" % (t.dtype, tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t).__name__))
-    if not t.is_cuda:
-        raise ValueError("%s must be on the GPU" % name)
+    _on(t, name, dev)
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError("%s must be contiguous along its last dimension" % name)
+
+
+def _out(t, dtype, shape, dev):
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError("out must be a contiguous %s tensor %s" % (dtype, shape))
+    _on(t, "out", dev)
+
+
+def _on(t, name, dev):
+    if t.get_device() != dev:
+        raise ValueError("%s must be on the current GPU, cuda:%d, not on %s" % (name, dev, t.device))
 
 
 class KV4Cache:
@@ -69,7 +81,9 @@ class KV4Cache:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.read(slots)
-        _need(slots, "slots", torch.int64, 1)
+        dev = torch.cuda.current_device()
+        _on(self.data, "the cache", dev)
+        _need(slots, "slots", torch.int64, 1, dev)
         T = slots.shape[0]
         k, v = slots.new_empty((2, T, self.NKV, self.HD), dtype=torch.float16).unbind(0)
         _ffi.call("ql_kv4_read", self.data.data_ptr(), self.num_pages, self.NKV, self.HD, self.page, self.group,
@@ -106,11 +120,12 @@ def plan(prev_lens, new_lens, block_table, free_pages, n_free, page, max_tokens,
     if stream is not None:
         with torch.cuda.stream(stream):              # what is allocated here belongs to it too
             return plan(prev_lens, new_lens, block_table, free_pages, n_free, page, max_tokens)
-    _need(prev_lens, "prev_lens", torch.int32, 1)
-    _need(new_lens, "new_lens", torch.int32, 1)
-    _need(block_table, "block_table", torch.int32, 2)
-    _need(free_pages, "free_pages", torch.int32, 1)
-    _need(n_free, "n_free", torch.int32, 1)
+    dev = torch.cuda.current_device()
+    _need(prev_lens, "prev_lens", torch.int32, 1, dev)
+    _need(new_lens, "new_lens", torch.int32, 1, dev)
+    _need(block_table, "block_table", torch.int32, 2, dev)
+    _need(free_pages, "free_pages", torch.int32, 1, dev)
+    _need(n_free, "n_free", torch.int32, 1, dev)
     n, width = block_table.shape
     if new_lens.shape[0] != n or prev_lens.shape[0] != n:
         raise ValueError("prev_lens, new_lens and block_table must have a row for each request: %d, %d, %d"
@@ -139,31 +154,33 @@ def qk_norm_rope(qkv, NH, NKV, HD, positions, cos, sin, *, q_weight=None, k_weig
         with torch.cuda.stream(stream):
             return qk_norm_rope(qkv, NH, NKV, HD, positions, cos, sin, q_weight=q_weight, k_weight=k_weight, eps=eps,
                                 cache=cache, slots=slots, out=out)
-    _need(qkv, "qkv", qkv.dtype, 2)
+    dev = torch.cuda.current_device()
+    _need(qkv, "qkv", qkv.dtype, 2, dev)
     T, width = qkv.shape
     if width != (NH + 2 * NKV) * HD:
         raise ValueError("qkv must be [T, %d], got %s" % ((NH + 2 * NKV) * HD, tuple(qkv.shape)))
-    _need(positions, "positions", torch.int32, 1)
-    _need(cos, "cos", torch.float32, 2)
-    _need(sin, "sin", torch.float32, 2)
+    _need(positions, "positions", torch.int32, 1, dev)
+    _need(cos, "cos", torch.float32, 2, dev)
+    _need(sin, "sin", torch.float32, 2, dev)
     lmax, half = cos.shape
     if positions.shape[0] != T or sin.shape != cos.shape or not cos.is_contiguous() or not sin.is_contiguous():
         raise ValueError("positions must be [T], cos and sin contiguous [lmax, rot / 2]")
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None:
-            _need(w, name, torch.float32, 1)
+            _need(w, name, torch.float32, 1, dev)
             if w.shape[0] != HD:
                 raise ValueError("%s must be [%d]" % (name, HD))
     if out is None:
         out = qkv.new_empty((T, NH, HD))
-    elif out.dtype != qkv.dtype or tuple(out.shape) != (T, NH, HD) or not out.is_contiguous():
-        raise ValueError("out must be a contiguous %s tensor %s" % (qkv.dtype, (T, NH, HD)))
+    else:
+        _out(out, qkv.dtype, (T, NH, HD), dev)
     k = None
     if cache is None:
         k = qkv.new_empty((T, NKV, HD))
         where = (k.data_ptr(), None, 0, 0, 0, None)
     else:
-        _need(slots, "slots", torch.int64, 1)
+        _need(slots, "slots", torch.int64, 1, dev)
+        _on(cache.data, "the cache", dev)
         if cache.NKV != NKV or cache.HD != HD or slots.shape[0] != T:
             raise ValueError("the cache holds %d heads of %d, and slots must be [T]" % (cache.NKV, cache.HD))
         where = (None, cache.data.data_ptr(), cache.num_pages, cache.page, cache.group, slots.data_ptr())
@@ -186,7 +203,9 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
     if stream is not None:
         with torch.cuda.stream(stream):
             return attention(q, cache, block_table, seq_lens, cu_q, scale=scale, window=window, out=out, workspace=workspace)
-    _need(q, "q", q.dtype, 3)
+    dev = torch.cuda.current_device()
+    _need(q, "q", q.dtype, 3, dev)
+    _on(cache.data, "the cache", dev)
     T, NH, HD = q.shape
     ldq = NH * HD
     dense = q.is_contiguous()
@@ -194,8 +213,8 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
         if q.stride(2) != 1 or q.stride(1) != HD:
             raise ValueError("q must be [T, NH, HD] with contiguous heads, got %s, strides %s" % (tuple(q.shape), q.stride()))
         ldq = q.stride(0)
-    _need(block_table, "block_table", torch.int32, 2)
-    _need(seq_lens, "seq_lens", torch.int32, 1)
+    _need(block_table, "block_table", torch.int32, 2, dev)
+    _need(seq_lens, "seq_lens", torch.int32, 1, dev)
     B, width = block_table.shape
     if HD != cache.HD or NH % cache.NKV or seq_lens.shape[0] != B:
         raise ValueError("q has %d heads of %d, the cache %d of %d; block_table has %d rows for %d requests"
@@ -204,18 +223,24 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
         if T < B:
             raise ValueError("%d queries for %d requests" % (T, B))
     else:
-        _need(cu_q, "cu_q", torch.int32, 1)
+        _need(cu_q, "cu_q", torch.int32, 1, dev)
         if cu_q.shape[0] != B + 1:
             raise ValueError("cu_q must be [%d]" % (B + 1))
     if q.data_ptr() % 16 or ldq * q.element_size() % 16:      # the kernel reads 16 bytes at a time
         q, ldq, dense = torch.empty((T, NH, HD), dtype=q.dtype, device=q.device).copy_(q), NH * HD, True
     if out is None:
         out = torch.empty_like(q) if dense else q.new_empty((T, NH, HD))
-    elif out.dtype != q.dtype or tuple(out.shape) != (T, NH, HD) or not out.is_contiguous():
-        raise ValueError("out must be a contiguous %s tensor %s" % (q.dtype, (T, NH, HD)))
-    ws = _attention_workspace(cache, NH) if workspace is None else workspace
+    else:
+        _out(out, q.dtype, (T, NH, HD), dev)
+    if workspace is None:
+        ws = _attention_workspace(cache, NH)
+    else:
+        ws = workspace
+        _on(ws, "workspace", dev)
+        if not ws.is_contiguous():
+            raise ValueError("workspace must be contiguous")
     _ffi.call("ql_kv4_attention", q.data_ptr(), _ffi.dtype_code(q.dtype), ldq, T, NH, cache.NKV, HD, cache.data.data_ptr(),
               cache.num_pages, cache.page, cache.group, block_table.data_ptr(), block_table.stride(0) if B > 1 else width,
               width, seq_lens.data_ptr(), _ffi.ptr(cu_q), B, HD ** -0.5 if scale is None else scale, window,
-              out.data_ptr(), ws.data_ptr(), ws.numel(), _ffi.stream_ptr(None, q.device))
+              out.data_ptr(), ws.data_ptr(), ws.nbytes, _ffi.stream_ptr(None, q.device))
     return out
