@@ -143,6 +143,13 @@ QL_API size_t ql_gptq_matmul_noalloc_max_scratch(void);
 QL_API int ql_device_status(void);
 
 /*
+ * The id of the capture that `stream` is in (a CUDA graph in the making), or 0: whoever keeps a workspace for
+ * each stream can tell the calls that a graph will replay, on whatever stream, from those that run there now.
+ * No counterpart in the reference.
+ */
+QL_API unsigned long long ql_stream_capture_id(void* stream);
+
+/*
  * Load-time row sort for act-order (desc_act) checkpoints: qweight_out row k' takes packed
  * value k = perm[k'] of qweight_in (both int32 [K/per, N]). With perm = a stable argsort of
  * g_idx, every group becomes a contiguous run of gs rows and ql_gptq_matmul(x_perm = perm)
@@ -410,9 +417,11 @@ QL_API int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, int pa
  * A row that sees no position is zero, and so are rows past cu_q[B]. A page id outside the cache or a
  * length past the table gives nan. Scores, softmax and sums are fp32; with 16-bit inputs of more than 8
  * rows (query tokens x NH / NKV) a request, probabilities are rounded to 11 bits, else to 22.
- * Workspace: ql_kv4_attention_workspace(NH, NKV, HD) bytes, 16-byte aligned, zeroed before the first call
- * (each call leaves its counters at zero); calls that share one must not overlap. out is 8-byte aligned.
+ * Workspace: ql_kv4_attention_workspace(NH, NKV, HD) bytes, 16-byte aligned, its first QL_KV4_COUNTER_BYTES (the
+ * counters) zeroed before the first call (each call leaves them at zero); calls that share one must not overlap, those
+ * that a graph replays among them. out is 8-byte aligned.
  */
+#define QL_KV4_COUNTER_BYTES 2048
 QL_API size_t ql_kv4_attention_workspace(int NH, int NKV, int HD);
 QL_API int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int NH, int NKV, int HD, const void* cache,
                      int num_pages, int page, int group, const int32_t* table, long table_stride, int table_width,

@@ -31,6 +31,7 @@ SIGNATURES = {
                                    _c_long, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp,
                                    ctypes.c_size_t, _vp]),
     "ql_device_status": (_c_int, []),
+    "ql_stream_capture_id": (ctypes.c_ulonglong, [_vp]),
     "ql_gptq_matmul_noalloc": (_c_int, [_vp, _c_int, _c_long, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int,
                                         _c_long, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp]),
     "ql_gptq_matmul_noalloc_max_scratch": (ctypes.c_size_t, []),

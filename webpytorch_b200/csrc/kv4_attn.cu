@@ -41,6 +41,7 @@ namespace {
 using namespace kv4;
 
 constexpr int kMaxCtas = 512;   // counters in the workspace
+static_assert(kMaxCtas * sizeof(unsigned int) == QL_KV4_COUNTER_BYTES, "the part of the workspace that callers zero");
 // Rows of a request from which the prompt kernel takes it: where the GPU is full, its tile pair costs
 // what 2.3 of the streaming kernel's 16-row tiles do. 200 requests of 3000 positions, 32 heads over 4: 48 rows 382 us
 // there, 355 here; 64 rows 384 and 450.

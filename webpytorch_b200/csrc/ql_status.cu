@@ -51,6 +51,13 @@ int env_int(const char* name, int dflt) {
 
 extern "C" int ql_set_launch_flags(int flags) { return ql::g_launch_flags.exchange(flags); }
 
+extern "C" unsigned long long ql_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) return 0;
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 extern "C" int ql_version(void) { return 100; }  // 0.1.0
 
 extern "C" const char* ql_last_error(void) { return ql::g_err; }

@@ -91,20 +91,34 @@ class KV4Cache:
         return k, v
 
 
-_workspaces = {}
+_workspaces = {}     # (GPU, HD, stream): the workspace of the calls on that stream
+_captured = {}       # the same: (capture, workspace) of the calls that a graph takes up there
+_COUNTER_BYTES = 2048                             # QL_KV4_COUNTER_BYTES
 
 
 def _attention_workspace(cache, NH):
     """The attention's workspace on the current stream, made once and shared by the layers' caches: its counters
-    are zero between calls, and calls that share one may not overlap."""
-    key = (cache.device.index, cache.HD, _ffi.stream_ptr(None, cache.device))
+    are zero between calls, and calls that share one may not overlap. A graph is replayed on any stream, beside
+    others, so the calls that it captures have a workspace of their own in the graph's memory, whose counters the
+    graph zeroes before the first of them."""
+    stream = _ffi.stream_ptr(None, cache.device)
+    key = (cache.device.index, cache.HD, stream)
+    if torch.cuda.is_current_stream_capturing():
+        capture = _ffi.fn("ql_stream_capture_id")(stream)
+        held = _captured.get(key)
+        if held is None or held[0] != capture:
+            held = _captured[key] = (capture, _new_workspace(cache, NH))
+        return held[1]
     ws = _workspaces.get(key)
     if ws is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("attention needs its workspace before a graph is captured: call it once on this "
-                               "stream first, or pass workspace=")
-        n = int(_ffi.fn("ql_kv4_attention_workspace")(NH, cache.NKV, cache.HD))
-        ws = _workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=cache.device)
+        ws = _workspaces[key] = _new_workspace(cache, NH)
+    return ws
+
+
+def _new_workspace(cache, NH):
+    n = int(_ffi.fn("ql_kv4_attention_workspace")(NH, cache.NKV, cache.HD))
+    ws = torch.empty(n, dtype=torch.uint8, device=cache.device)
+    ws[:_COUNTER_BYTES].zero_()
     return ws
 
 
@@ -198,7 +212,7 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
     cu_q[b + 1] - 1 are request b's last tokens (cu_q int32 [B + 1]; None: one token each). block_table
     int32 [B, width], seq_lens int32 [B] with those tokens counted. window: positions that a query sees
     (0: all). workspace: uint8 of ql_kv4_attention_workspace bytes, zeroed once and not shared by calls that
-    overlap (None: one for each stream). Rows that see nothing, and rows past cu_q[B], are zero. Returns
+    overlap (None: one for each stream, and one for each graph that is captured there). Rows that see nothing, and rows past cu_q[B], are zero. Returns
     [T, NH, HD] in q's dtype."""
     if stream is not None:
         with torch.cuda.stream(stream):
