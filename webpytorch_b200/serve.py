@@ -25,7 +25,8 @@ class ServeStack:
     """layers: DecodeLayers; head_norms: None, or for each layer (q_weight, k_weight) fp32 [HD].
 
     `requests` rows of lengths and block tables, `pages` pages of `page` positions in each layer's cache
-    (4.5 bits a value at group 64), at most `lmax` positions a request and `cap` <= 16 tokens a step."""
+    (4.5 bits a value at group 64), at most `lmax` positions a request (rounded up to whole pages: attribute `lmax`) and
+    `cap` <= 16 tokens a step. A request that asks for more is not served and keeps its length."""
 
     def __init__(self, layers, H, NH, NKV, HD, lmax, requests, pages, page=64, group=64, cap=16, theta=1e6, eps=1e-6,
                  head_norms=None, device=None, graph=True):
@@ -34,6 +35,8 @@ class ServeStack:
         if head_norms is not None and len(head_norms) != len(layers):
             raise ValueError("head_norms must have an entry for each of the %d layers" % len(layers))
         self.layers, self.H, self.NH, self.NKV, self.HD = layers, H, NH, NKV, HD
+        width = -(-lmax // page)
+        lmax = width * page                        # what the plan serves, and so what the rotation's tables cover
         self.lmax, self.requests, self.cap, self.eps, self.page = lmax, requests, cap, float(eps), page
         dev = self.dev = layers[0].qkv.qweight.device if device is None else torch.device(device)
         self.head_norms = [(None, None)] * len(layers) if head_norms is None else [
@@ -41,7 +44,7 @@ class ServeStack:
         self.caches = [kv4.KV4Cache(pages, NKV, HD, page=page, group=group, device=dev) for _ in layers]
         i32 = dict(dtype=torch.int32, device=dev)
         self.lens = torch.zeros(requests, **i32)
-        self.table = torch.full((requests, -(-lmax // page)), -1, **i32)
+        self.table = torch.full((requests, width), -1, **i32)
         self.free = torch.arange(pages - 1, -1, -1, **i32)
         self.n_free = torch.tensor([pages], **i32)
         self.new = torch.zeros(requests, **i32)
