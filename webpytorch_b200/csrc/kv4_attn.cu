@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
     uint32_t src;
     int pos[R];
     float coef[R];
-    bool bad;
+    bool bad[R];                                // nan: for this lane's rows
     {
       Request r = c.r;
       int b = c.b;
@@ -588,9 +588,11 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
       n = max(min(r.blo + (int)(end - item0), (hi_all + kBlock - 1) / kBlock) - blk0, 0);
       first_masked = (p_first + 1) / kBlock - blk0;
       first_seen = a.window ? (max(p_last - a.window + 1, 0) + kBlock - 1) / kBlock - blk0 : 0;
-      bad = r.seq > table_end;                  // a length past the table: nan
 #pragma unroll
-      for (int i = 0; i < R; ++i) pos[i] = r.seq - r.ql + (r0 + min(g + 8 * i, nrows - 1)) / grp;
+      for (int i = 0; i < R; ++i) {
+        pos[i] = r.seq - r.ql + (r0 + min(g + 8 * i, nrows - 1)) / grp;
+        bad[i] = r.seq > table_end;             // a length past the table
+      }
       __syncwarp();
       if (lane == 0) {
         c.r = r;
@@ -632,7 +634,8 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
       if (!warp_wait(bar + 8 * s, phase, &abort_flag) ||
           (both && !warp_wait(bar + 8 * s1, phase ^ (s1 == 0), &abort_flag))) {
         // gave up: nan for this tile, and no copy left in flight
-        bad = true;
+#pragma unroll
+        for (int j = 0; j < R; ++j) bad[j] = true;
         for (int j = i; j < min(i + ST, n); ++j) {
           ptx::mbar_wait_drain(bar + 8 * s, phase);
           if (++s == ST) s = 0, phase ^= 1;
@@ -640,22 +643,25 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
         __syncwarp();
         break;
       }
-      // a page that is not one of the cache's: nan
-      bad = bad || ((missing >> (i & 31)) & 1) || (both && ((missing >> (i & 31)) & 2));
+      const uint32_t gone = (missing >> (i & 31)) & (both ? 3u : 1u);   // blocks whose page is not one of the cache's
       const uint8_t* const blk[2] = {ring + s * BB, ring + s1 * BB};
-      if (i >= first_seen && i + 1 < first_masked && both) {
+      if (i >= first_seen && i + 1 < first_masked && both && !gone) {
         const int all[R] = {};
         attend_blocks<HD, G, PL, false>(st, blk, qf, coef, all, all, 0, 2 * kBlock);
       } else {
-        // (of a second block past the last one nothing is seen)
-        const int p0 = (blk0 + i) * kBlock, end = both ? 2 * kBlock : kBlock;
+        // (of a second block past the last one nothing is seen, and nothing of one that is gone: the rows that would
+        // see it are nan)
+        const int p0 = (blk0 + i) * kBlock, from = gone & 1 ? kBlock : 0, to = both && !(gone & 2) ? 2 * kBlock : kBlock;
         int lo[R], hi[R];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
           lo[j] = (a.window ? max(pos[j] - a.window + 1, 0) : 0) - p0;
-          hi[j] = min(pos[j] + 1 - p0, end);
+          hi[j] = pos[j] + 1 - p0;
+          bad[j] = bad[j] || ((gone & 1) && lo[j] < kBlock && hi[j] > 0) || ((gone & 2) && lo[j] < 2 * kBlock && hi[j] > kBlock);
+          lo[j] = max(lo[j], from);
+          hi[j] = min(hi[j], to);
         }
-        attend_blocks<HD, G, PL, true>(st, blk, qf, coef, lo, hi, c.lo_all - p0, min(c.hi_all - p0, end));
+        attend_blocks<HD, G, PL, true>(st, blk, qf, coef, lo, hi, max(c.lo_all - p0, from), min(c.hi_all - p0, to));
       }
       __syncwarp();
       // the stages are free: blocks i + ST and i + ST + 1 go there
@@ -668,7 +674,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
     for (int i = 0; i < R; ++i) {
       st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 1);
       st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 2);
-      if (bad) st.l[i] = __int_as_float(0x7fc00000);
+      if (bad[i]) st.l[i] = __int_as_float(0x7fc00000);
     }
     if (c.item0 >= c.u0 && c.item1 <= c.u1) {
       write_tile<DT, HD, PL>(a, st, c.r.q0, c.kvh, c.r0, c.nrows, grp);

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     ptx::mbar_init(done, 1);
     for (int i = 0; i < kDecodeWarps * kRing; ++i) ptx::mbar_init(bar0 + 8u * (L::kRingBar + i), 1);
     *abort_flag = 0;
-    *bad_flag = seq > table_end;                  // a length past the table: nan
+    *bad_flag = 0;
     ptx::fence_mbar_init();
   }
   if (warp == kWarps - 1) {
@@ -336,7 +336,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     }
     if (steps > 0 && ok) ok = warp_wait(done, 0, ab);
     ptx::tc_fence_after();
-    if (*bad_flag || !ok) run.l = __int_as_float(0x7fc00000);
+    bool bad = !ok || seq > table_end;            // a length past the table: nan
+    if (*bad_flag)                                // pages that are not the cache's: nan for the rows that see one
+      for (int p = row_lo >> a.page_shift; p <= min(pos, table_end - 1) >> a.page_shift; ++p)
+        bad = bad || (unsigned)a.table[b * a.table_stride + p] >= (unsigned)a.num_pages;
+    if (bad) run.l = __int_as_float(0x7fc00000);
     const float inv = CUT ? 1.f : run.l == 0.f ? 0.f : 1.f / run.l;   // a row that sees nothing is zero
     float4* part = CUT ? reinterpret_cast<float4*>(part_of<HD>(a, blockIdx.y, blockIdx.x, gridDim.x)) : nullptr;
     if (CUT) reinterpret_cast<float2*>(part + HD / 4 * kRows)[i] = make_float2(run.m, run.l);
@@ -433,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
           }
           if (have && ((missing >> (bn & 31)) & 1)) {
             have = false;
-            if (lane == 0) *bad_flag = 1;          // a page that is not one of the cache's: nan
+            if (lane == 0) *bad_flag = 1;          // a page that is not one of the cache's
           }
           const unsigned char* blk = raw + (bn % kRing) * BB + (kv ? code_bytes(HD) + scale_bytes(HD, G) : 0);
 #pragma unroll
