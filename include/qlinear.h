@@ -414,8 +414,9 @@ QL_API int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, int pa
  *   q [T][NH][HD] of dtype, token stride ldq (heads contiguous, tokens 16-byte aligned); out [T][NH][HD] of dtype
  *   table int32 [B][table_width], row stride table_stride; window 0, or the number of positions that a
  *   query sees, its own the last
- * A row that sees no position is zero, and so are rows past cu_q[B]. A page id outside the cache or a
- * length past the table gives nan. Scores, softmax and sums are fp32; with 16-bit inputs of more than 8
+ * A row that sees no position is zero, and so are rows past cu_q[B]. A page id outside the cache gives nan to the
+ * rows that see the page, a length past the table to all rows of the request; keys and values that are not finite reach
+ * the rows that see them and no others. Scores, softmax and sums are fp32; with 16-bit inputs of more than 8
  * rows (query tokens x NH / NKV) a request, probabilities are rounded to 11 bits, else to 22.
  * Workspace: ql_kv4_attention_workspace(NH, NKV, HD) bytes, 16-byte aligned, its first QL_KV4_COUNTER_BYTES (the
  * counters) zeroed before the first call (each call leaves them at zero); calls that share one must not overlap, those

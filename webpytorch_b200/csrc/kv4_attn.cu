@@ -186,17 +186,117 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, const Request& r
 constexpr float kLazy = 6.f;
 constexpr float kPShift = 9.f;   // p' = 2^9 p, up to 2^15: 11 bits of probabilities down to 2^-23
 
+// O += P V of a block's values vc, for P's fragment p; any_lo / any_hi: the positions of the block that some row sees. In a
+// masked block values that are not finite are looked for first: where there are any, true is returned and nothing is
+// added. ODD: they count as zero.
+template <int HD, int G, bool MASKED, bool ODD>
+__device__ __forceinline__ bool add_values(float (&o)[HD / 8][4], const uint32_t (&p)[4], const uint8_t* vc, int any_lo,
+                                           int any_hi) {
+  constexpr int VW = HD / 64;               // words of a lane and position
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const __half2* vs = reinterpret_cast<const __half2*>(vc + code_bytes(HD));
+  // words of positions t, t + 4 | t + 8, t + 12, elements g HD / 8 ...
+  uint32_t w[4][VW];
+  __half2 s2[2], m2[2], sm[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint8_t* from = vc + (t + 4 * k) * (HD / 2) + g * (HD / 16);
+    if constexpr (VW == 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(from);
+      w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
+    } else if constexpr (VW == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(from);
+      w[k][0] = u.x; w[k][1] = u.y;
+    } else {
+      w[k][0] = *reinterpret_cast<const uint32_t*>(from);
+    }
+    sm[k] = vs[(t + 4 * k) * (HD / G) + g * (HD / 8) / G];
+  }
+  if (MASKED) {
+    bool odd = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (t + 4 * k < any_lo || t + 4 * k >= any_hi) sm[k] = h2_const(0u);
+      odd = odd || may_not_be_finite(sm[k]);
+    }
+    if (!ODD && __any_sync(0xffffffffu, odd)) return true;
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    s2[k] = __lows2half2(sm[2 * k], sm[2 * k + 1]);
+    m2[k] = __highs2half2(sm[2 * k], sm[2 * k + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < VW; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t sel = h ? 0x7632u : 0x5410u;
+      __half2 b0[4], b1[4];
+      // nibbles 0..3 of the half words of two positions: codes_h2 reads the interleaved word as
+      // (nibble j of one, nibble j of the other)
+      codes_h2(__byte_perm(w[0][i], w[1][i], sel), b0);
+      codes_h2(__byte_perm(w[2][i], w[3][i], sel), b1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        b0[k] = __hfma2(b0[k], s2[0], m2[0]);
+        b1[k] = __hfma2(b1[k], s2[1], m2[1]);
+        if (ODD) {
+          b0[k] = finite_or_zero(b0[k]);
+          b1[k] = finite_or_zero(b1[k]);
+        }
+        mma_16816_f16(o[8 * i + 4 * h + k], p[0], p[1], p[2], p[3], h2_as_u32(b0[k]), h2_as_u32(b1[k]));
+      }
+    }
+  return false;
+}
+
+// The same for a masked block with values that are not finite: they count as zero in the product, whose rows share
+// them, and 0 x, which is nan for them and 0 for all others, is added for the rows that see the position. lo / hi: of this
+// lane's rows, relative to the block. Called, not inlined, so that it takes no registers from the loop.
+template <int HD, int G, int PL>
+__device__ __noinline__ void add_odd_values(float (&o)[HD / 8][4], uint32_t p0, uint32_t p1, uint32_t p2, uint32_t p3,
+                                            const uint8_t* vc, int any_lo, int any_hi, int2 row0, int2 row1) {
+  const uint32_t p[4] = {p0, p1, p2, p3};
+  add_values<HD, G, true, true>(o, p, vc, any_lo, any_hi);
+  const __half2* vs = reinterpret_cast<const __half2*>(vc + code_bytes(HD));
+  const int t = threadIdx.x & 3;
+#pragma unroll 1
+  for (int at = 0; at < kBlock; ++at) {
+    const bool sees[2] = {at >= row0.x && at < row0.y, at >= row1.x && at < row1.y};
+    if (!sees[0] && !sees[1]) continue;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {           // the lane's elements t HD / 4 ...; element e is in tile e % (HD / 8)
+      const __half2 sm = vs[at * (HD / G) + (t * (HD / 4) + 8 * j) / G];
+      __half2 n[4];
+      codes_h2(*reinterpret_cast<const uint32_t*>(vc + at * (HD / 2) + t * (HD / 8) + 4 * j), n);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 x = __half22float2(__hfma2(n[q], __low2half2(sm), __high2half2(sm)));
+        const int i = (8 * j + q) % (HD / 8), k = 8 * j / (HD / 8);
+#pragma unroll
+        for (int r = 0; r < 3 - PL; ++r) {
+          float &a = o[i][2 * r + k], &b = o[i + 4][2 * r + k];
+          a = sees[r] ? fmaf(0.f, x.x, a) : a;
+          b = sees[r] ? fmaf(0.f, x.y, b) : b;
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
+
 // Two blocks of 16 positions in shared memory: what there is once for a step of the loop (waits, the maximum's
 // shuffles and vote) is once for 32 positions. MASKED: some of them are not seen by some row. lo / hi: visible
 // positions of this lane's rows, relative to the first block; any_lo / any_hi: of any row. A masked position
 // has p = 0, and where no row sees it its scales are dropped too, since memory that was never written may
-// hold codes for nan.
+// hold codes for nan. Where some rows see it and it is not finite, the product takes it as zero for all of them, and the
+// rows that do see it are given nan after it.
 template <int HD, int G, int PL, bool MASKED>
 __device__ __forceinline__ void attend_blocks(State<HD, PL>& st, const uint8_t* const (&blk)[2], const uint4* qf,
                                               const float (&coef)[3 - PL], const int (&lo)[3 - PL],
                                               const int (&hi)[3 - PL], int any_lo, int any_hi) {
   constexpr int R = 3 - PL;                 // rows of a lane
-  constexpr int KW = HD / 32, VW = HD / 64; // words of a lane: keys of one position, values of one
+  constexpr int KW = HD / 32;               // words of a lane and position
   constexpr int NG = HD / G, TWO = HD == 256 && G == 32 ? 2 : 1;   // groups that a lane's key elements are in
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float z[R][8];                            // S of positions 16 b + t + 4 k, at 4 b + k
@@ -308,54 +408,23 @@ __device__ __forceinline__ void attend_blocks(State<HD, PL>& st, const uint8_t* 
       }
     }
   }
-  // values: words of positions t, t + 4 | t + 8, t + 12, elements g HD / 8 ...
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
     const uint8_t* vc = blk[b] + code_bytes(HD) + scale_bytes(HD, G);
-    const uint8_t* vs = vc + code_bytes(HD);
-    uint32_t w[4][VW];
-    __half2 s2[2], m2[2], sm[4];
+    const bool odd = add_values<HD, G, MASKED, false>(st.o, a[b], vc, any_lo - 16 * b, any_hi - 16 * b);
+    if (MASKED && odd) {
+      float o[HD / 8][4];                       // a copy that has an address
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint8_t* p = vc + (t + 4 * k) * (HD / 2) + g * (HD / 16);
-      if constexpr (VW == 4) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
-      } else if constexpr (VW == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[k][0] = u.x; w[k][1] = u.y;
-      } else {
-        w[k][0] = *reinterpret_cast<const uint32_t*>(p);
-      }
-      sm[k] = reinterpret_cast<const __half2*>(vs)[(t + 4 * k) * NG + g * (HD / 8) / G];
+      for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = st.o[i][j];
+      add_odd_values<HD, G, PL>(o, a[b][0], a[b][1], a[b][2], a[b][3], vc, any_lo - 16 * b, any_hi - 16 * b,
+                                make_int2(lo[0] - 16 * b, hi[0] - 16 * b), make_int2(lo[R - 1] - 16 * b, hi[R - 1] - 16 * b));
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) st.o[i][j] = o[i][j];
     }
-    if (MASKED) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (16 * b + t + 4 * k < any_lo || 16 * b + t + 4 * k >= any_hi) sm[k] = h2_const(0u);
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      s2[k] = __lows2half2(sm[2 * k], sm[2 * k + 1]);
-      m2[k] = __highs2half2(sm[2 * k], sm[2 * k + 1]);
-    }
-#pragma unroll
-    for (int i = 0; i < VW; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t sel = h ? 0x7632u : 0x5410u;
-        __half2 b0[4], b1[4];
-        // nibbles 0..3 of the half words of two positions: codes_h2 reads the interleaved word as
-        // (nibble j of one, nibble j of the other)
-        codes_h2(__byte_perm(w[0][i], w[1][i], sel), b0);
-        codes_h2(__byte_perm(w[2][i], w[3][i], sel), b1);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          b0[k] = __hfma2(b0[k], s2[0], m2[0]);
-          b1[k] = __hfma2(b1[k], s2[1], m2[1]);
-          mma_16816_f16(st.o[8 * i + 4 * h + k], a[b][0], a[b][1], a[b][2], a[b][3], h2_as_u32(b0[k]), h2_as_u32(b1[k]));
-        }
-      }
   }
 }
 

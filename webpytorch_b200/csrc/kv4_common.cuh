@@ -43,5 +43,20 @@ __device__ __forceinline__ void codes_h2(uint32_t w, __half2 (&out)[4]) {
   out[3] = __hfma2(u32_as_h2(lop3_andor(u, 0x00F000F0u, kMagicF16x2)), k16, k64);
 }
 
+// Whether some value of a group with (s, m) may not be finite: a group that stands for nan, or a last code past
+// fp16's range.
+__device__ __forceinline__ bool may_not_be_finite(__half2 sm) {
+  const __half top = __hfma(__habs(__low2half(sm)), __ushort_as_half((unsigned short)0x4B80), __habs(__high2half(sm)));   // 15 |s| + |m|
+  return (__half_as_ushort(top) & 0x7fffu) >= 0x7c00u;
+}
+
+// A pair of values, those that are not finite as zero.
+__device__ __forceinline__ __half2 finite_or_zero(__half2 v) {
+  uint32_t u = h2_as_u32(v);
+  if ((u & 0x7c00u) == 0x7c00u) u &= 0xffff0000u;
+  if ((u & 0x7c000000u) == 0x7c000000u) u &= 0x0000ffffu;
+  return u32_as_h2(u);
+}
+
 }  // namespace kv4
 }  // namespace ql

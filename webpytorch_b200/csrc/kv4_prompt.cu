@@ -22,6 +22,8 @@
 // tokens over 2500 to 6000 positions (32 heads over 4, HD 128, bf16), which take 259 us, 600 TFLOP/s. A step of
 // 128 positions takes a CTA 2.2 us: one exponential a score and the decoding of the codes fill the issue slots
 // beside the tensor work, and 370 pairs of tiles over 148 SMs leave the last wave half empty.
+#include <type_traits>
+
 #include "kv4_common.cuh"
 #include "kv4_attn.cuh"
 #include "sm100_ptx.cuh"
@@ -52,7 +54,8 @@ struct Smem {
   static constexpr int kRingBar = 20;
   static constexpr int kBars = kRingBar + kDecodeWarps * kRing;
   static constexpr int kMisc = kBar + kBars * 8;
-  static constexpr int kBytes = kMisc + 16 + 1024;   // + alignment slack
+  static constexpr int kItem = kMisc + 16;
+  static constexpr int kBytes = kItem + 32 + 1024;   // + alignment slack
 };
 
 // Chunk (16 bytes, one word of 8 codes) of a row: word w of the row is at panel, column.
@@ -86,6 +89,106 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 constexpr float kLazy = 6.f, kPShift = 9.f;      // as in the streaming kernel
+
+constexpr int kRows = kTiles * kTileRows;
+
+// Pair of tiles `item` of `items`, tiles of the longest rows first: rows r0 .. r0 + nrows - 1 of request b and a
+// key/value head. nrows is 0 for one past a request's last row, or of a request that is not the prompt kernel's.
+struct Item {
+  int b, kvh, q0, ql, r0, nrows;
+};
+__device__ __forceinline__ Item item_at(const AttnArgs& a, int grp, int item, int items) {
+  Item it;
+  it.kvh = item % a.NKV;
+  const int x = items / a.NKV - 1 - item / a.NKV;
+  const auto tile_start = [&](int b) { return (int)((long)cu(a, b) * grp / kRows) + b; };
+  it.b = 0;
+  for (int hi = a.B - 1; it.b < hi;) {            // the last request whose first pair of tiles is at or before x
+    const int mid = (it.b + hi + 1) >> 1;
+    if (tile_start(mid) <= x) it.b = mid;
+    else hi = mid - 1;
+  }
+  it.q0 = cu(a, it.b);
+  it.ql = max(cu(a, it.b + 1) - it.q0, 0);
+  const int rows = it.ql * grp;
+  it.r0 = (x - tile_start(it.b)) * kRows;
+  it.nrows = rows < a.prompt_rows || it.r0 >= rows ? 0 : min(kRows, rows - it.r0);
+  return it;
+}
+
+// The rare paths of the kernel are functions that are called and find the row again, so that they take no registers
+// from it: positions lo .. hi - 1 that row i of a pair of tiles sees, and those that all of its rows see.
+struct Sight {
+  int lo, hi, common_lo, common_hi;
+};
+__device__ __forceinline__ Sight sight_of(const AttnArgs& a, const Item& it, int i) {
+  const int grp = a.NH / a.NKV, p0 = max(a.seq_lens[it.b], 0) - it.ql;
+  const auto lo = [&](int p) { return a.window ? max(p - a.window + 1, 0) : 0; };
+  const int pos = p0 + (it.r0 + min(i, it.nrows - 1)) / grp;
+  return {lo(pos), min(pos + 1, a.width << a.page_shift), lo(p0 + (it.r0 + it.nrows - 1) / grp), p0 + it.r0 / grp + 1};
+}
+
+// Whether row i sees a page that is not the cache's.
+__device__ __noinline__ bool sees_bad_page(const AttnArgs& a, const Item& it, int i) {
+  const Sight see = sight_of(a, it, i);
+  bool bad = false;
+  for (int p = see.lo >> a.page_shift; p <= (see.hi - 1) >> a.page_shift; ++p)
+    bad = bad || (unsigned)a.table[it.b * a.table_stride + p] >= (unsigned)a.num_pages;
+  return bad;
+}
+
+// 32 codes of a position, words 4 t .. 4 t + 3 of row `row`, into a tile of keys or values. FINITE: values that are not
+// count as zero.
+template <int HD, bool FINITE>
+__device__ __forceinline__ void decode_words(unsigned char* to, int row, int t, uint4 u, __half2 sm) {
+  const __half2 s2 = __low2half2(sm), m2 = __high2half2(sm);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __half2 h[4];
+    codes_h2(w[i], h);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      h[q] = __hfma2(h[q], s2, m2);
+      if (FINITE) h[q] = finite_or_zero(h[q]);
+    }
+    const int word = 4 * t + i;
+    *reinterpret_cast<uint4*>(to + panel_of<HD>(word) * (128 * 128) + row * 128 + ((column_of<HD>(word) ^ (row & 7)) << 4)) =
+        make_uint4(h2_as_u32(h[0]), h2_as_u32(h[1]), h2_as_u32(h[2]), h2_as_u32(h[3]));
+  }
+}
+template <int HD>
+__device__ __noinline__ void decode_finite(unsigned char* to, int row, int t, uint4 u, __half2 sm) {
+  decode_words<HD, true>(to, row, t, u, sm);
+}
+
+// Columns 32 k .. of row i's output in tensor-memory order: 0 x, which is nan for values that are not finite and 0 for all
+// others, is added for the positions that the row sees, but for those that all rows see, whose values were taken as they
+// are.
+template <int HD, int G>
+__device__ __noinline__ void add_odd_values(const AttnArgs& a, const Item& it, int i, int k, uint32_t (&v)[32]) {
+  const Sight see = sight_of(a, it, i);
+#pragma unroll 1
+  for (int p = see.lo; p < see.hi; ++p) {
+    if (p >= see.common_lo && p < see.common_hi) continue;
+    const uint32_t src = source(a, it.b, it.kvh, p >> 4, 0, 1);
+    if (src == kNoBlock) continue;
+    const uint8_t* vc = a.cache + (size_t)src * block_bytes(HD, G) + code_bytes(HD) + scale_bytes(HD, G);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int pc = 4 * k + c, w = HD == 64 ? pc : 4 * ((pc & 7) >> 1) + 2 * (pc >> 3) + (pc & 1);
+      const __half2 sm = reinterpret_cast<const __half2*>(vc + code_bytes(HD))[(p & 15) * (HD / G) + 8 * w / G];
+      __half2 n[4];
+      codes_h2(*reinterpret_cast<const uint32_t*>(vc + (p & 15) * (HD / 2) + 4 * w), n);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 x = __half22float2(__hfma2(n[q], __low2half2(sm), __high2half2(sm)));
+        v[8 * c + 2 * q] = __float_as_uint(fmaf(0.f, x.x, __uint_as_float(v[8 * c + 2 * q])));
+        v[8 * c + 2 * q + 1] = __float_as_uint(fmaf(0.f, x.y, __uint_as_float(v[8 * c + 2 * q + 1])));
+      }
+    }
+  }
+}
 
 // A row's running maximum (units of log2) and sum.
 struct Row {
@@ -166,32 +269,6 @@ __device__ __forceinline__ bool softmax_half(Row& row, uint32_t s_col, uint32_t 
   return true;
 }
 
-constexpr int kRows = kTiles * kTileRows;
-
-// Pair of tiles `item` of `items`, tiles of the longest rows first: rows r0 .. r0 + nrows - 1 of request b and a
-// key/value head. nrows is 0 for one past a request's last row, or of a request that is not the prompt kernel's.
-struct Item {
-  int b, kvh, q0, ql, r0, nrows;
-};
-__device__ __forceinline__ Item item_at(const AttnArgs& a, int grp, int item, int items) {
-  Item it;
-  it.kvh = item % a.NKV;
-  const int x = items / a.NKV - 1 - item / a.NKV;
-  const auto tile_start = [&](int b) { return (int)((long)cu(a, b) * grp / kRows) + b; };
-  it.b = 0;
-  for (int hi = a.B - 1; it.b < hi;) {            // the last request whose first pair of tiles is at or before x
-    const int mid = (it.b + hi + 1) >> 1;
-    if (tile_start(mid) <= x) it.b = mid;
-    else hi = mid - 1;
-  }
-  it.q0 = cu(a, it.b);
-  it.ql = max(cu(a, it.b + 1) - it.q0, 0);
-  const int rows = it.ql * grp;
-  it.r0 = (x - tile_start(it.b)) * kRows;
-  it.nrows = rows < a.prompt_rows || it.r0 >= rows ? 0 : min(kRows, rows - it.r0);
-  return it;
-}
-
 // A part of a pair of tiles: HD / 4 x kRows fours of O (a row's four to a lane, so that lanes store and load next
 // to each other), then (m, l) of the rows.
 template <int HD>
@@ -206,7 +283,7 @@ __device__ __forceinline__ float* part_of(const AttnArgs& a, int split, int item
 // heads over 4: 119 us whole, 47 cut; 64 tokens 117 and 34. One kernel for both took 266 us where the whole
 // one takes 260.)
 template <int DT, int HD, int G, bool CUT>
-__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_constant__ AttnArgs a) {
   using L = Smem<HD, G>;
   constexpr int BB = block_bytes(HD, G), W = HD / 8;
   const int grp = a.NH / a.NKV;
@@ -238,6 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
   volatile int* bad_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 8);
+  volatile int* odd_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 12);
+  Item* kept_item = reinterpret_cast<Item*>(smem + L::kItem);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // uniform
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -256,6 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     for (int i = 0; i < kDecodeWarps * kRing; ++i) ptx::mbar_init(bar0 + 8u * (L::kRingBar + i), 1);
     *abort_flag = 0;
     *bad_flag = 0;
+    *odd_flag = 0;
+    *kept_item = item;
     ptx::fence_mbar_init();
   }
   if (warp == kWarps - 1) {
@@ -337,20 +418,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     if (steps > 0 && ok) ok = warp_wait(done, 0, ab);
     ptx::tc_fence_after();
     bool bad = !ok || seq > table_end;            // a length past the table: nan
-    if (*bad_flag)                                // pages that are not the cache's: nan for the rows that see one
-      for (int p = row_lo >> a.page_shift; p <= min(pos, table_end - 1) >> a.page_shift; ++p)
-        bad = bad || (unsigned)a.table[b * a.table_stride + p] >= (unsigned)a.num_pages;
+    if (*bad_flag) bad = bad || sees_bad_page(a, *kept_item, i);
     if (bad) run.l = __int_as_float(0x7fc00000);
     const float inv = CUT ? 1.f : run.l == 0.f ? 0.f : 1.f / run.l;   // a row that sees nothing is zero
     float4* part = CUT ? reinterpret_cast<float4*>(part_of<HD>(a, blockIdx.y, blockIdx.x, gridDim.x)) : nullptr;
     if (CUT) reinterpret_cast<float2*>(part + HD / 4 * kRows)[i] = make_float2(run.m, run.l);
     uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + ((long)tok * a.NH + head) * HD;
+    const bool odd = *odd_flag;
 #pragma unroll
     for (int k = 0; k < HD / 32; ++k) {
       uint32_t v[32];
       if (steps > 0) {
         ptx::tmem_ld32(o_col + 32u * k, v);
         ptx::tmem_wait_ld();
+      }
+      if (odd && steps > 0) {
+        uint32_t x[32];                           // a copy that has an address
+#pragma unroll
+        for (int c = 0; c < 32; ++c) x[c] = v[c];
+        add_odd_values<HD, G>(a, *kept_item, i, k, x);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = x[c];
+        __syncwarp();
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {               // columns 8 (4 k + c) ...: one word's elements
@@ -392,6 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
     const unsigned char* raw = smem + L::kRaw + d * kRing * BB;
     constexpr int LP = HD / 32, PW = 32 / LP;     // lanes of a position, positions of a pass
     const int t = lane % LP, pr = lane / LP;
+    const int common_lo = a.window ? max(p_last - a.window + 1, 0) : 0;   // all rows see common_lo .. p_first
     // the warp's blocks in order: n-th is block d + 4 n of the item. Lane i looks up block i of the next 32.
     const int mine = nblk > d ? (nblk - d + 3) / 4 : 0;
     const auto lookup = [&](int n) { return n < mine ? source(a, b, kvh, blk0, d + 4 * n, nblk) : kNoBlock; };
@@ -440,32 +530,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnArgs a) {
             if (lane == 0) *bad_flag = 1;          // a page that is not one of the cache's
           }
           const unsigned char* blk = raw + (bn % kRing) * BB + (kv ? code_bytes(HD) + scale_bytes(HD, G) : 0);
+          // values that some row does not see: its p = 0 would make nan of one that is not finite
+          const int start = (blk0 + 8 * j + d + 4 * half) * kBlock;
+          const bool edge = kv == 1 && (start + kBlock - 1 > p_first || start < common_lo);
+          // a loop for each, since the check within one takes the large calls from 301 to 311 us
+          const auto passes = [&](auto at_edge) {
 #pragma unroll
-          for (int pass = 0; pass < kBlock / PW; ++pass) {
-            const int p = pass * PW + pr, at = (2 * 4 * j + d + 4 * half) * kBlock + p;   // in the block, in the item
-            const int row = (d + 4 * half) * kBlock + p;
-            const int seen = blk0 * kBlock + at;
-            uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            __half2 sm = h2_const(0u);
-            // positions that no row sees are zero: their memory may never have been written
-            if (have && seen >= lo_all && seen < hi_all) {
-              u = *reinterpret_cast<const uint4*>(blk + p * (HD / 2) + t * 16);
-              sm = reinterpret_cast<const __half2*>(blk + code_bytes(HD))[p * (HD / G) + t * 32 / G];
+            for (int pass = 0; pass < kBlock / PW; ++pass) {
+              const int p = pass * PW + pr, at = (2 * 4 * j + d + 4 * half) * kBlock + p;   // in the block, in the item
+              const int row = (d + 4 * half) * kBlock + p;
+              const int seen = blk0 * kBlock + at;
+              uint4 u = make_uint4(0u, 0u, 0u, 0u);
+              __half2 sm = h2_const(0u);
+              // positions that no row sees are zero: their memory may never have been written
+              if (have && seen >= lo_all && seen < hi_all) {
+                u = *reinterpret_cast<const uint4*>(blk + p * (HD / 2) + t * 16);
+                sm = reinterpret_cast<const __half2*>(blk + code_bytes(HD))[p * (HD / G) + t * 32 / G];
+              }
+              if (decltype(at_edge)::value && (seen > p_first || seen < common_lo) && may_not_be_finite(sm)) {
+                *odd_flag = 1;
+                decode_finite<HD>(to, row, t, u, sm);
+              } else {
+                decode_words<HD, false>(to, row, t, u, sm);
+              }
             }
-            const __half2 s2 = __low2half2(sm), m2 = __high2half2(sm);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              __half2 h[4];
-              codes_h2(w[i], h);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) h[q] = __hfma2(h[q], s2, m2);
-              const int word = 4 * t + i;
-              *reinterpret_cast<uint4*>(to + panel_of<HD>(word) * L::kPanel + row * 128 +
-                                        ((column_of<HD>(word) ^ (row & 7)) << 4)) =
-                  make_uint4(h2_as_u32(h[0]), h2_as_u32(h[1]), h2_as_u32(h[2]), h2_as_u32(h[3]));
-            }
-          }
+          };
+          if (edge) passes(std::true_type());
+          else passes(std::false_type());
           if (kv == 1 && bn < mine) {              // the block's values were its last part
             __syncwarp();
             ++n;
