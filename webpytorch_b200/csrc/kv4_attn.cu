@@ -1048,7 +1048,7 @@ extern "C" int ql_kv4_attention(const void* q, int dtype, long ldq, int T, int N
   a.cu_q = cu_q;
   a.B = B;
   a.scale = scale;
-  a.window = window;
+  a.window = window < table_width * page ? window : 0;   // one as long as the table hides nothing
   a.prompt_rows = prompts_pay(T, B, NH, HD, dtype) ? kPromptRows : 0;
   a.out = out;
   a.counters = reinterpret_cast<unsigned int*>(workspace);

@@ -26,6 +26,8 @@ from .qlinear import _device
 
 __all__ = ["KV4Cache", "Plan", "plan", "qk_norm_rope", "attention"]
 
+_INT_MAX = 2 ** 31 - 1
+
 Plan = namedtuple("Plan", "seq_lens cu_new slots positions requests n_free")
 
 
@@ -255,6 +257,6 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
             raise ValueError("workspace must be contiguous")
     _ffi.call("ql_kv4_attention", q.data_ptr(), _ffi.dtype_code(q.dtype), ldq, T, NH, cache.NKV, HD, cache.data.data_ptr(),
               cache.num_pages, cache.page, cache.group, block_table.data_ptr(), block_table.stride(0) if B > 1 else width,
-              width, seq_lens.data_ptr(), _ffi.ptr(cu_q), B, HD ** -0.5 if scale is None else scale, window,
+              width, seq_lens.data_ptr(), _ffi.ptr(cu_q), B, HD ** -0.5 if scale is None else scale, min(window, _INT_MAX),
               out.data_ptr(), ws.data_ptr(), ws.nbytes, _ffi.stream_ptr(None, q.device))
     return out
