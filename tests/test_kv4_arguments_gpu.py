@@ -1,8 +1,10 @@
-"""Arguments at the ends of their ranges: windows as long as any number."""
+"""Arguments at the ends of their ranges: windows as long as any number, queries of one head with any stride."""
+import numpy as np
 import pytest
 import torch
 
-from test_kv4_gpu import Batch, attend
+from test_kv4_gpu import Batch, attend, dev
+from webpytorch_b200 import kv4
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +24,15 @@ def test_a_window_past_every_position_hides_nothing(dtype, HD, NH, NKV, lens, ql
         assert torch.equal(got, want)
     else:
         bt.check(q, cu, got, dtype, window)
+
+
+def test_one_head_in_rows_that_are_wider():
+    bt = Batch([20, 33], 1, 64, 16, 32, 22)
+    q, cu = bt.queries([2, 3], 1, "bf16")
+    wide = torch.full((5, 64 + 24), float("nan"), dtype=torch.bfloat16, device="cuda")
+    wide[:, :64] = q[:, 0]
+    want = attend(bt, q, cu)
+    bt.check(q, cu, want, "bf16")
+    for strided in (wide[:, None, :64], wide.as_strided((5, 1, 64), (88, 8, 1)), wide.as_strided((5, 1, 64), (88, 0, 1))):
+        got = kv4.attention(strided, bt.cache, bt.table, dev(bt.lens), dev(cu))
+        assert torch.equal(got, want) and np.isfinite(got.float().cpu().numpy()).all()

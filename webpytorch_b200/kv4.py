@@ -226,7 +226,7 @@ def attention(q, cache, block_table, seq_lens, cu_q=None, *, scale=None, window=
     ldq = NH * HD
     dense = q.is_contiguous()
     if not dense:
-        if q.stride(2) != 1 or q.stride(1) != HD:
+        if q.stride(2) != 1 or (NH > 1 and q.stride(1) != HD):
             raise ValueError("q must be [T, NH, HD] with contiguous heads, got %s, strides %s" % (tuple(q.shape), q.stride()))
         ldq = q.stride(0)
     _need(block_table, "block_table", torch.int32, 2, dev)
