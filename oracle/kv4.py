@@ -74,17 +74,6 @@ def values(codes, s, m):
     return v.reshape(*v.shape[:-2], -1)
 
 
-def pack_block(kc, ks, km, vc, vs, vm):
-    """The bytes of blocks of 16 positions: codes [..., 16, groups, G], s and m [..., 16, groups]."""
-    out = []
-    for c, s, m in ((kc, ks, km), (vc, vs, vm)):
-        c = c.reshape(*c.shape[:-2], -1)
-        out.append((c[..., 0::2] | c[..., 1::2] << 4).reshape(*c.shape[:-2], -1))
-        sm = np.stack([s, m], -1).astype(np.float16)
-        out.append(np.ascontiguousarray(sm.reshape(*sm.shape[:-3], -1)).view(np.uint8))
-    return np.concatenate(out, -1)
-
-
 def attention(q, K, V, cu, lens, scale, window=0):
     """q [T, NH, HD]; K, V lists of [len, NKV, HD]; causal from the end of each request, in 64 bits."""
     out = np.zeros(q.shape)
