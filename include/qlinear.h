@@ -353,7 +353,8 @@ QL_API int ql_moe_combine(const float* z, const int32_t* pair_row, const float* 
  *   K codes [16][HD / 2] | K (s, m) [16][HD / group] | V codes [16][HD / 2] | V (s, m) [16][HD / group]
  * two codes to a byte (LSB first), (s, m) pairs of halves. For each group of elements of a position
  * m = half(min), s = half((max - min) / 15), n = rint((x - m) / s) in 0 .. 15, and a code stands for
- * half(s n + m); a group with an input that is not finite (or beyond 65504) stands for nan. Slot i is
+ * half(s n + m); a group with an input that is not finite (or beyond 65504) stands for nan. (The last code of a group
+ * within a rounding of +-65504 can stand for infinity.) Slot i is
  * position i % page of page i / page. HD is 64, 128 or 256, page a power of two from 16 to 4096, group
  * 32, 64 or 128 and at most HD; other sizes are refused.
  * --------------------------------------------------------------------------------------- */
@@ -417,7 +418,8 @@ QL_API int ql_kv4_read(const void* cache, int num_pages, int NKV, int HD, int pa
  * A row that sees no position is zero, and so are rows past cu_q[B]. A page id outside the cache gives nan to the
  * rows that see the page, a length past the table to all rows of the request; keys and values that are not finite reach
  * the rows that see them and no others. Scores, softmax and sums are fp32; with 16-bit inputs of more than 8
- * rows (query tokens x NH / NKV) a request, probabilities are rounded to 11 bits, else to 22.
+ * rows (query tokens x NH / NKV) a request on average (T over B, rows past cu_q[B] counted in) probabilities are
+ * rounded to 11 bits, else to 22, as are fp32 queries.
  * Workspace: ql_kv4_attention_workspace(NH, NKV, HD) bytes, 16-byte aligned, its first QL_KV4_COUNTER_BYTES (the
  * counters) zeroed before the first call (each call leaves them at zero); calls that share one must not overlap, those
  * that a graph replays among them. out is 8-byte aligned.

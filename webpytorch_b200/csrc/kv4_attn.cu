@@ -6,8 +6,8 @@
 // rows, r = i (NH / NKV) + head; a tile takes the next rows of it. The warp MMA (m16n8k16, fp16 in,
 // fp32 out) has 16 of them. One-plane tiles use them for 16 rows; two-plane tiles hold 8 rows as
 // fp16 high and low parts (22 bits), rows r and r + 8 of the MMA, whose results the same thread
-// holds and adds: fp32 queries and probabilities keep fp32 accuracy, and tiles of 8 rows or fewer
-// pay nothing for it.
+// holds and adds: queries and probabilities keep 22 bits. Tiles of 8 rows or fewer take as many MMAs as one plane
+// would; of 16-bit queries, which one plane holds exactly, the low parts are zeros.
 // Keys. A lane owns HD / 4 consecutive elements of a position (a 16-byte load at HD = 128), all in
 // one group of at least 32 elements, so a scale pair is loaded once per position. The order of the
 // contraction is free, so the pairs the nibble masks give (element j with j + 4 of a word) are the
@@ -24,11 +24,11 @@
 // a tile to be joined: first with the parts of the CTA's other warps, then, for at most two tiles a
 // CTA, with those of other CTAs by whichever of them finishes last, always in the same order.
 // Bound. A position is NKV (HD + 8 HD / G) bytes, and each of its 4-bit codes is unpacked once by one lane: about
-// 13 instructions for 8 codes, of which 5 are the ALU pipe's. Long ragged batches run at 45 % of the measured copy
-// rate, held by that pipe and the MMAs (45 and 32 % busy over the whole call; a busy pipe is what warps wait for
-// most): 96 requests of 200 to 12000 positions (8 heads of 128, 320 MB) 109 us, 2.9 TB/s; 131071 positions of one
-// request (4 heads, 71 MB) 41 us. Short calls are the fixed chain: launch and first loads 8 us, the join in a CTA 3,
-// across CTAs 3 (513 positions 14 us).
+// 13 instructions for 8 codes, of which 5 are the ALU pipe's. Long ragged batches run at 42 % of the measured copy
+// rate, and no pipe is full over the whole call (ALU 46 %, tensor 32 %, issue slots 57 %); fixed latencies and busy
+// pipes are what warps wait for most: 96 requests of 200 to 12000 positions (8 heads of 128, 303 MB) 110 us, 2.75 TB/s;
+// 131071 positions of one request (4 heads, 71 MB) 43 us. Short calls are the fixed chain: launch and first loads 8 us,
+// the join in a CTA 3, across CTAs 3 (513 positions 15 us).
 #include "kv4_attn.cuh"
 
 namespace ql {
@@ -44,7 +44,7 @@ constexpr int kMaxCtas = 512;   // counters in the workspace
 static_assert(kMaxCtas * sizeof(unsigned int) == QL_KV4_COUNTER_BYTES, "the part of the workspace that callers zero");
 // Rows of a request from which the prompt kernel takes it: where the GPU is full, its tile pair costs
 // what 2.3 of the streaming kernel's 16-row tiles do. 200 requests of 3000 positions, 32 heads over 4: 48 rows 382 us
-// there, 355 here; 64 rows 384 and 450.
+// there, 360 here; 64 rows 415 and 449.
 constexpr int kPromptRows = 64;
 
 // Warps of a CTA by the registers that a head's state takes, and ring stages by what they leave.
@@ -917,10 +917,12 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1) kv4_attention_kernel(A
 
 // Whether requests of kPromptRows rows or more are the prompt kernel's. It takes 16 positions of 16 rows in a
 // fifth of the streaming kernel's time (0.16 against 0.8 ns over all SMs at HD = 128), and costs a join and another
-// launch, so it pays from some rows on. The host knows the tokens past one a request. Measured, both sides,
-// bf16: 32 heads of 128 over 4, 6000 positions, 17 tokens 31 us (streaming 32), 32 35 (38), 64 35 (53), 256 48 (151), 2000
-// 204 (1014); 64 tokens over 64 positions 21 (18), over 1000 27 (28); 8 requests of 8 tokens 35 (37), of 32 48 (90); 16
-// heads of 64, 3000 positions: 64 tokens 25 (23), 256 32 (35).
+// launch, so it pays from some rows on. The host knows the tokens past one a request, and not how they are spread.
+// Measured, both sides, bf16: 32 heads of 128 over 4, 6000 positions, 64 tokens 36 us (streaming 56), 256 49 (152), 2000
+// 211 (1039); 64 tokens over 64 positions 22 (18), over 1000 27 (29); 8 requests of 8 tokens 37 (39), of 32 49 (90); 16
+// heads of 64, 3000 positions: 64 tokens 24 (24), 256 33 (37). Where no request has the rows after all, the launch costs 8
+// to 16 us: 64 requests of 4000 positions, 2 tokens each 83 (70), 32 heads over 8 and 3 tokens 126 (110). The same tokens
+// may be one chunk beside decoding requests, which wins more than that.
 bool prompts_pay(int T, int B, int NH, int HD, int dtype) {
   return dtype != QL_F32 && HD <= 128 && (long)(T - B) * NH * HD >= 1l << 17;
 }
@@ -962,8 +964,8 @@ template <int DT, int HD, int G>
 int launch(const AttnArgs& a, int ctas, cudaStream_t st) {
   // One plane where 16-bit inputs fill more than 8 rows of a tile: their outputs keep no more than the 11 bits of a
   // single fp16 probability. The host knows the mean only. Measured, 64 requests of 4000 positions, bf16, HD = 128,
-  // one plane (two planes): 32 heads over 8, 1 token 103 us (99), 3 tokens 107 (183); over 4, 1 token 62 (58),
-  // 2 tokens 66 (100). HD = 256, 32 requests: 32 over 4, 1 token 63.6 (63.4), 2 tokens 80 (101).
+  // one plane (two planes): 32 heads over 8, 1 token 103 us (98), 3 tokens 126 (189); over 4, 1 token 62 (59),
+  // 2 tokens 83 (104). HD = 256, 32 requests: 32 over 4, 1 token 67 (67), 2 tokens 84 (103).
   constexpr bool can = DT != QL_F32;
   if (can && (long)a.T * (a.NH / a.NKV) > 8L * a.B) return launch_one<DT, HD, G, can ? 1 : 2>(a, ctas, st);
   return launch_one<DT, HD, G, 2>(a, ctas, st);

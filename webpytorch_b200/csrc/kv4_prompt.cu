@@ -18,10 +18,12 @@
 // the same layout read as MN-major for P V. The order of a position's elements is free (the contraction of
 // S; the columns of O), so it is the one in which a lane's 16-byte load of 32 codes gives four 16-byte
 // stores without bank conflicts.
-// Bound. 4 NH HD operations a visible (query, position): 93.5 us at the measured rate for two chunks of 900 to 2000
-// tokens over 2500 to 6000 positions (32 heads over 4, HD 128, bf16), which take 259 us, 600 TFLOP/s. A step of
-// 128 positions takes a CTA 2.2 us: one exponential a score and the decoding of the codes fill the issue slots
-// beside the tensor work, and 370 pairs of tiles over 148 SMs leave the last wave half empty.
+// Bound. 4 NH HD operations a visible (query, position): chunks of 900 and 2000 tokens over 6000 and 3340 positions (32
+// heads over 4, HD 128, bf16) are 159 GFLOP, 95 us at the measured rate, and take 231 us, 685 TFLOP/s. A step of 128
+// positions takes a CTA about 4200 clocks, of which the exponentials (16 a clock and SM) and the tensor work are 2048
+// each: no pipe is full (tensor 38 %, XU 38 %, issue slots 45 %), and what warps wait for most is loads from tensor
+// memory, two for each score. 13 warps leave a thread 128 registers, and at HD 128 some are spilled. 368 pairs of
+// tiles over 148 SMs leave the last wave half empty.
 #include <type_traits>
 
 #include "kv4_common.cuh"
@@ -280,8 +282,7 @@ __device__ __forceinline__ float* part_of(const AttnArgs& a, int split, int item
 
 // CUT: where a call has at most half as many pairs of tiles as the GPU has SMs, the positions of a pair are cut
 // into gridDim.y equal pieces, and prompt_join_kernel adds up what they leave. (256 tokens over 6000 positions, 32
-// heads over 4: 119 us whole, 47 cut; 64 tokens 117 and 34. One kernel for both took 266 us where the whole
-// one takes 260.)
+// heads over 4: 119 us whole, 49 cut; 64 tokens 117 and 36. One kernel for both was 2 % slower on large calls.)
 template <int DT, int HD, int G, bool CUT>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const __grid_constant__ AttnArgs a) {
   using L = Smem<HD, G>;
